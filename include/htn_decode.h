@@ -511,6 +511,70 @@ int htn_xcc_ids(int32_t* out, int64_t blocks, htn_stream_t stream);
 int htn_attention_merge_in_kernel(void);
 int htn_attention_disable_in_kernel_merge(void);
 
+/* ---------------------------------------------------------------- paged cache
+ *
+ * No counterpart in the reference, whose cache is one contiguous block per
+ * sequence. The pools keys and values hold pages of page_size slots (a power
+ * of two, 16 to 1024): [pages, Hkv, page_size, 128] bf16, 16-byte aligned. Slot
+ * s of sequence b is row s % page_size of page page_table[b * table_st +
+ * s / page_size], s / page_size < table_pages (at most 2^29 slots). Sequence b's
+ * new tokens are rows starts[b] .. starts[b + 1] - 1 of the packed inputs
+ * (starts holds batch + 1 values), the last of them at position
+ * lengths[b] - 1: lengths counts the new tokens. All four arrays are read on
+ * the device. starts must not fall and must lie within [0, tokens], else the
+ * attention writes nothing (the append takes the sequences that do lie there). A
+ * sequence whose length is negative or does not fit its table sees nothing and
+ * stores nothing, as does a row before slot 0. A page id outside [0, pages)
+ * reads as zeros and is not written; entries of slots that no row sees are not
+ * used. Output rows of no sequence are left as they were. */
+
+/* The new tokens' q, k (heads packed, 128 wide, row strides given, multiples of
+ * 8) normalised per head (x gain / sqrt(mean(x^2) + eps); a NULL gain leaves
+ * that one unnormalised) and rotated by the cos/sin table row of their position
+ * (bf16, or fp32 with rope_fp32; row stride a multiple of 8; zeros for a
+ * position past rope_rows), in fp32 and rounded once; q to out_q
+ * [tokens, Hq, 128], k and v to their cache slots. */
+int htn_norm_rope_paged(const void* q, int64_t q_st, const void* k, int64_t k_st,
+                        const void* v, int64_t v_st, const void* q_gain, const void* k_gain,
+                        float q_eps, float k_eps, const void* cos, const void* sin,
+                        int64_t rope_st, int64_t rope_rows, int rope_fp32, void* keys,
+                        void* values, int64_t pages, int64_t page_size,
+                        const int32_t* page_table, int64_t table_st, int64_t table_pages,
+                        const int64_t* starts, const int64_t* lengths, int64_t batch,
+                        int64_t tokens, int64_t q_heads, int64_t kv_heads, void* out_q,
+                        htn_stream_t stream);
+
+/* out[t, h] = softmax(q . k / sqrt(128)) v over the slots s <= p, p the row's
+ * position; with window > 0 of these only s > p - window and s < sinks. Rows
+ * that see nothing get zeros. Infinities and NaN in slots that a row does not
+ * see do not reach it. q and out rows at t * st + h * sh elements (q strides
+ * multiples of 8 from a 16-byte aligned base, out strides of 4 from an 8-byte
+ * aligned one). scratch: htn_paged_attention_scratch_bytes bytes, no initial
+ * contents, 16-byte aligned. */
+int64_t htn_paged_attention_scratch_bytes(int64_t tokens, int64_t batch, int64_t q_heads,
+                                          int64_t kv_heads, int shared_prefix);
+int htn_paged_attention(const void* q, int64_t q_st, int64_t q_sh, const void* keys,
+                        const void* values, int64_t pages, int64_t page_size,
+                        const int32_t* page_table, int64_t table_st, int64_t table_pages,
+                        const int64_t* starts, const int64_t* lengths, int64_t window,
+                        int64_t sinks, void* out, int64_t o_st, int64_t o_sh, int64_t batch,
+                        int64_t tokens, int64_t q_heads, int64_t kv_heads, void* scratch,
+                        int64_t scratch_bytes, htn_stream_t stream);
+
+/* The same without a window, where slots below prefix_length[0] (taken within
+ * [0, prefix_count * page_size]) are those of prefix_pages for every sequence:
+ * their K and V are read once for all rows, and the sequences' own table
+ * entries of whole pages below it are not used. */
+int htn_shared_prefix_attention(const void* q, int64_t q_st, int64_t q_sh, const void* keys,
+                                const void* values, int64_t pages, int64_t page_size,
+                                const int32_t* prefix_pages, int64_t prefix_count,
+                                const int64_t* prefix_length, const int32_t* page_table,
+                                int64_t table_st, int64_t table_pages, const int64_t* starts,
+                                const int64_t* lengths, void* out, int64_t o_st, int64_t o_sh,
+                                int64_t batch, int64_t tokens, int64_t q_heads,
+                                int64_t kv_heads, void* scratch, int64_t scratch_bytes,
+                                htn_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
