@@ -167,9 +167,10 @@ def prepare(case, seed):
     else:
         state.q = normal(total, heads, D, std=2.0).to(torch.bfloat16)
     if case["kind"] == "prefix":
-        # The prefix's last page may hold the first sequence's own slots too.
-        state.prefix_pages = table[0, :-(-prefix // page)].contiguous()
-        state.prefix_length = torch.tensor([prefix], device=DEVICE)
+        # Whole pages are shared; the rest of a prefix that ends inside a page lies
+        # in pages of the sequences' own.
+        state.prefix_pages = table[0, :max(1, shared)].contiguous()
+        state.prefix_length = torch.tensor([shared * page], device=DEVICE)
     return state
 
 
