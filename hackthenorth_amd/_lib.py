@@ -97,6 +97,9 @@ SIGNATURES = {
     "htn_shared_prefix_attention": [_P, _I64, _I64, _P, _P, _I64, _I64, _P, _I64, _P, _P, _I64,
                                     _I64, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _P,
                                     _I64, _P],
+    "htn_sample_scratch_bytes": [_I64, _I64],
+    "htn_sample": [_P, _I64, _I, _I64, _I64, _P, _P, _F, _P, _I64, _P, _F, _P, _F, _P, _P, _I64,
+                   _P],
     "htn_xcc_ids": [_P, _I64, _P],
     "htn_attention_merge_in_kernel": [],
     "htn_attention_disable_in_kernel_merge": [],
@@ -106,7 +109,8 @@ RESTYPES = {"htn_attention_scratch_bytes": _I64, "htn_gemm_rows_scratch_bytes": 
             "htn_gemm_library_workspace_bytes": _I64,
             "htn_gate_up_swiglu_scratch_bytes": _I64, "htn_stream_read_blocks": _I64,
             "htn_attention_output_scratch_bytes": _I64, "htn_attention_output_fused_calls": _I64,
-            "htn_paged_attention_scratch_bytes": _I64, "htn_head_scratch_capacity": _I64}
+            "htn_paged_attention_scratch_bytes": _I64, "htn_sample_scratch_bytes": _I64,
+            "htn_head_scratch_capacity": _I64}
 EPI_STORE, EPI_RESIDUAL, EPI_SWIGLU, EPI_ARGMAX, EPI_RESIDUAL_NORM = 0, 1, 2, 3, 4
 
 _lib = None
