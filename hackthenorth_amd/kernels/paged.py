@@ -18,54 +18,75 @@ nothing and stores nothing. Page ids outside the pool read as zeros and are not
 written, and entries of slots that no row sees are never used. Rows of no
 sequence (behind the last one in a padded batch) are left as they were.
 """
-import contextlib
+import functools
 
 import torch
 
 from .. import _lib
 
-
-def _on(device):
-    """The device of the tensors as the current one, for the launch."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+_BF16, _I32, _I64 = torch.bfloat16, torch.int32, torch.int64
+_PAGES = tuple(16 << i for i in range(7))
 
 
-def _check_pools(key_pages, value_pages, kv_heads):
-    if key_pages.shape != value_pages.shape or key_pages.dim() != 4 \
-            or key_pages.shape[0] < 1 or key_pages.shape[1] != kv_heads \
-            or key_pages.shape[3] != _lib.HEAD_DIM or not key_pages.is_contiguous() \
-            or not value_pages.is_contiguous() or key_pages.dtype != torch.bfloat16 \
-            or value_pages.dtype != torch.bfloat16:
+def _place(first, *others):
+    """The index of the GPU that all the tensors are on (None ones aside)."""
+    index = first.get_device()
+    if index < 0:
+        _lib.require_gpu(first)
+    for t in others:
+        if t is not None and t.get_device() != index:
+            _lib.require_gpu(t)
+            raise ValueError("all tensors must be on one device")
+    return index
+
+
+def _launch(name, index, *args):
+    """The library call on the current stream of GPU `index`, current for the launch."""
+    if index == torch.cuda.current_device():
+        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+
+
+def _check_pools(key_pages, value_pages):
+    """(pages, kv heads, page size)"""
+    shape = key_pages.shape
+    if len(shape) != 4 or value_pages.shape != shape or shape[3] != _lib.HEAD_DIM or 0 in shape \
+            or key_pages.dtype is not _BF16 or value_pages.dtype is not _BF16 \
+            or not key_pages.is_contiguous() or not value_pages.is_contiguous():
         raise ValueError("page pools must be contiguous bf16 [pages, Hkv, page_size, 128]")
-    page = key_pages.shape[2]
-    if page < 16 or page > 1024 or page & (page - 1):
+    if shape[2] not in _PAGES:
         raise ValueError("page_size must be a power of two from 16 to 1024")
+    return shape[:3]
 
 
 def _check_batch(page_table, query_starts, lengths):
-    if page_table.dim() != 2 or page_table.dtype != torch.int32 or 0 in page_table.shape \
-            or page_table.stride(1) != 1:
+    """(batch, row stride of the table, its pages)"""
+    shape, strides = page_table.shape, page_table.stride()
+    if len(shape) != 2 or page_table.dtype is not _I32 or 0 in shape or strides[1] != 1:
         raise ValueError("page_table must be int32 [B, P] with unit column stride")
-    batch = page_table.shape[0]
-    if query_starts.dtype != torch.int64 or query_starts.shape != (batch + 1,) \
+    batch = shape[0]
+    if query_starts.dtype is not _I64 or query_starts.shape != (batch + 1,) \
             or not query_starts.is_contiguous():
         raise ValueError("query_starts must be contiguous int64 with one entry per sequence and one more")
-    if lengths.dtype != torch.int64 or lengths.shape != (batch,) or not lengths.is_contiguous():
+    if lengths.dtype is not _I64 or lengths.shape != (batch,) or not lengths.is_contiguous():
         raise ValueError("lengths must be contiguous int64 with one entry per sequence")
-
-
-def _check_device(first, *others):
-    _lib.require_gpu(first, *others)
-    if any(t is not None and t.device != first.device for t in others):
-        raise ValueError("all tensors must be on one device")
+    return batch, strides[0], shape[1]
 
 
 def _rows(t, name):
-    if t.dim() != 3 or t.dtype != torch.bfloat16 or t.shape[2] != _lib.HEAD_DIM \
-            or t.stride(2) != 1:
+    """Shape and strides of packed rows."""
+    shape, strides = t.shape, t.stride()
+    if len(shape) != 3 or t.dtype is not _BF16 or shape[2] != _lib.HEAD_DIM or strides[2] != 1:
         raise ValueError(f"{name} must be bf16 [T, heads, 128] with unit dim stride")
+    return shape, strides
+
+
+@functools.lru_cache(maxsize=256)
+def _scratch_bytes(tokens, batch, heads, kv_heads, shared):
+    return max(16, _lib.load().htn_paged_attention_scratch_bytes(tokens, batch, heads, kv_heads,
+                                                                 shared))
 
 
 def norm_rope_paged(q, k, v, q_norm, k_norm, cos, sin, key_pages, value_pages, page_table,
@@ -78,75 +99,72 @@ def norm_rope_paged(q, k, v, q_norm, k_norm, cos, sin, key_pages, value_pages, p
     head; None leaves both unnormalised. Norm and rotation run in fp32 and round
     once, where norm_rope_cache keeps the reference's rounding after every step.
     """
-    for t, name in ((q, "q"), (k, "k"), (v, "v")):
-        _rows(t, name)
-        if t.shape[1] > 1 and t.stride(1) != _lib.HEAD_DIM:
+    (shape, q_st), (k_shape, k_st), (v_shape, v_st) = _rows(q, "q"), _rows(k, "k"), _rows(v, "v")
+    tokens, heads, dim = shape
+    kv_heads = k_shape[1]
+    for name, count, strides in (("q", heads, q_st), ("k", kv_heads, k_st), ("v", v_shape[1], v_st)):
+        if strides[1] != dim and count > 1:
             raise ValueError(f"{name} must have packed heads")
-    tokens, heads, _ = q.shape
-    if k.shape[0] != tokens or v.shape != k.shape:
+    if k_shape[0] != tokens or v_shape != k_shape:
         raise ValueError("q, k and v must share the tokens, k and v the heads")
-    if 0 in q.shape or 0 in k.shape:
+    if 0 in shape or kv_heads == 0:
         raise ValueError("q and k need tokens and heads")
-    if (q_norm is None) != (k_norm is None):
+    if q_norm is None and k_norm is None:
+        q_gain, k_gain, q_eps, k_eps = None, None, 0.0, 0.0
+    elif q_norm is None or k_norm is None:
         raise ValueError("q and k are both normalised or neither")
-    gains = (None, None) if q_norm is None else (q_norm.weight, k_norm.weight)
-    for g in gains:
-        if g is not None and (g.dtype != torch.bfloat16 or g.shape != (_lib.HEAD_DIM,)
-                              or not g.is_contiguous()):
-            raise ValueError("norm gains must be contiguous bf16 [128]")
-    if cos.shape != sin.shape or cos.dim() != 2 or cos.shape[1] != _lib.HEAD_DIM \
-            or cos.shape[0] < 1 or cos.dtype != sin.dtype \
-            or cos.dtype not in (torch.bfloat16, torch.float32) or cos.stride(1) != 1 \
-            or cos.stride() != sin.stride():
+    else:
+        q_gain, k_gain = q_norm.weight, k_norm.weight
+        q_eps, k_eps = float(q_norm.variance_epsilon), float(k_norm.variance_epsilon)
+        for g in (q_gain, k_gain):
+            if g.dtype is not _BF16 or g.shape != (dim,) or not g.is_contiguous():
+                raise ValueError("norm gains must be contiguous bf16 [128]")
+    table_shape, table_st, kind = cos.shape, cos.stride(), cos.dtype
+    if len(table_shape) != 2 or sin.shape != table_shape or table_shape[1] != dim \
+            or table_shape[0] < 1 or sin.dtype is not kind or kind not in (_BF16, torch.float32) \
+            or table_st[1] != 1 or sin.stride() != table_st:
         raise ValueError("cos/sin must be matching [positions, 128] tables, bf16 or fp32")
-    _check_pools(key_pages, value_pages, k.shape[1])
-    _check_batch(page_table, query_starts, lengths)
-    _check_device(q, k, v, *gains, cos, sin, key_pages, value_pages, page_table, query_starts,
-                  lengths)
-    out = torch.empty((tokens, heads, _lib.HEAD_DIM), dtype=q.dtype, device=q.device)
-    eps = (0.0, 0.0) if q_norm is None else (float(q_norm.variance_epsilon),
-                                             float(k_norm.variance_epsilon))
-    with _on(q.device):
-        _lib.call("htn_norm_rope_paged", _lib.ptr(q), q.stride(0), _lib.ptr(k), k.stride(0),
-                  _lib.ptr(v), v.stride(0), _lib.ptr(gains[0]), _lib.ptr(gains[1]), *eps,
-                  _lib.ptr(cos), _lib.ptr(sin), cos.stride(0), cos.shape[0],
-                  int(cos.dtype == torch.float32), _lib.ptr(key_pages), _lib.ptr(value_pages),
-                  key_pages.shape[0], key_pages.shape[2], _lib.ptr(page_table),
-                  page_table.stride(0), page_table.shape[1], _lib.ptr(query_starts),
-                  _lib.ptr(lengths), page_table.shape[0], tokens, heads, k.shape[1],
-                  _lib.ptr(out), _lib.stream(q.device))
-    return out
-
-
-def _attention_args(q, key_pages, value_pages, page_table, query_starts, lengths, out):
-    _rows(q, "q")
-    if 0 in q.shape:
-        raise ValueError("q needs tokens and heads")
-    tokens, heads, _ = q.shape
-    if key_pages.dim() != 4 or key_pages.shape[1] < 1 or heads % key_pages.shape[1]:
-        raise ValueError("query heads must be a multiple of kv heads")
-    _check_pools(key_pages, value_pages, key_pages.shape[1])
-    _check_batch(page_table, query_starts, lengths)
-    if out is None:
-        out = torch.empty((tokens, heads, _lib.HEAD_DIM), dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1:
-        raise ValueError("out must be a bf16 view shaped like q with unit dim stride")
+    pages, pool_heads, page = _check_pools(key_pages, value_pages)
+    if pool_heads != kv_heads:
+        raise ValueError("page pools must have k's heads")
+    batch, row_st, row_pages = _check_batch(page_table, query_starts, lengths)
+    index = _place(q, k, v, q_gain, k_gain, cos, sin, key_pages, value_pages, page_table,
+                   query_starts, lengths)
+    out = torch.empty(shape, dtype=_BF16, device=q.device)
+    _launch("htn_norm_rope_paged", index, q.data_ptr(), q_st[0], k.data_ptr(), k_st[0],
+            v.data_ptr(), v_st[0], _lib.ptr(q_gain), _lib.ptr(k_gain), q_eps, k_eps,
+            cos.data_ptr(), sin.data_ptr(), table_st[0], table_shape[0], kind is torch.float32,
+            key_pages.data_ptr(), value_pages.data_ptr(), pages, page, page_table.data_ptr(),
+            row_st, row_pages, query_starts.data_ptr(), lengths.data_ptr(), batch, tokens, heads,
+            kv_heads, out.data_ptr())
     return out
 
 
 def _attend(name, q, key_pages, value_pages, prefix, page_table, query_starts, lengths, mask, out):
-    tokens, heads, _ = q.shape
-    batch, kv_heads = page_table.shape[0], key_pages.shape[1]
-    nbytes = _lib.load().htn_paged_attention_scratch_bytes(tokens, batch, heads, kv_heads,
-                                                           int(bool(prefix)))
-    scratch = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=q.device)
-    with _on(q.device):
-        _lib.call(name, _lib.ptr(q), q.stride(0), q.stride(1), _lib.ptr(key_pages),
-                  _lib.ptr(value_pages), key_pages.shape[0], key_pages.shape[2], *prefix,
-                  _lib.ptr(page_table), page_table.stride(0), page_table.shape[1],
-                  _lib.ptr(query_starts), _lib.ptr(lengths), *mask, _lib.ptr(out), out.stride(0),
-                  out.stride(1), batch, tokens, heads, kv_heads, _lib.ptr(scratch), nbytes,
-                  _lib.stream(q.device))
+    shape, strides = _rows(q, "q")
+    if 0 in shape:
+        raise ValueError("q needs tokens and heads")
+    tokens, heads, _ = shape
+    pages, kv_heads, page = _check_pools(key_pages, value_pages)
+    if heads % kv_heads:
+        raise ValueError("query heads must be a multiple of kv heads")
+    batch, row_st, row_pages = _check_batch(page_table, query_starts, lengths)
+    if out is not None and (out.shape != shape or out.dtype is not _BF16 or out.stride(2) != 1):
+        raise ValueError("out must be a bf16 view shaped like q with unit dim stride")
+    index = _place(q, key_pages, value_pages, page_table, query_starts, lengths, out, *prefix)
+    device = q.device
+    if out is None:
+        out = torch.empty(shape, dtype=_BF16, device=device)
+        out_t, out_h = heads * _lib.HEAD_DIM, _lib.HEAD_DIM
+    else:
+        out_t, out_h, _ = out.stride()
+    nbytes = _scratch_bytes(tokens, batch, heads, kv_heads, bool(prefix))
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    before = (prefix[0].data_ptr(), prefix[0].numel(), prefix[1].data_ptr()) if prefix else ()
+    _launch(name, index, q.data_ptr(), strides[0], strides[1], key_pages.data_ptr(),
+            value_pages.data_ptr(), pages, page, *before, page_table.data_ptr(), row_st, row_pages,
+            query_starts.data_ptr(), lengths.data_ptr(), *mask, out.data_ptr(), out_t, out_h,
+            batch, tokens, heads, kv_heads, scratch.data_ptr(), nbytes)
     return out
 
 
@@ -164,8 +182,6 @@ def paged_attention(q, key_pages, value_pages, page_table, query_starts, lengths
         raise ValueError("window and sinks must not be negative")
     if sinks and not window:
         raise ValueError("sinks go with a window")
-    out = _attention_args(q, key_pages, value_pages, page_table, query_starts, lengths, out)
-    _check_device(q, key_pages, value_pages, page_table, query_starts, lengths, out)
     return _attend("htn_paged_attention", q, key_pages, value_pages, (), page_table, query_starts,
                    lengths, (int(window), int(sinks)), out)
 
@@ -186,9 +202,5 @@ def shared_prefix_attention(q, key_pages, value_pages, prefix_pages, prefix_leng
         raise ValueError("prefix_pages must be contiguous int32 [P]")
     if prefix_length.dtype != torch.int64 or prefix_length.numel() != 1:
         raise ValueError("prefix_length must be one int64")
-    out = _attention_args(q, key_pages, value_pages, page_table, query_starts, lengths, out)
-    _check_device(q, key_pages, value_pages, prefix_pages, prefix_length, page_table,
-                  query_starts, lengths, out)
-    prefix = (_lib.ptr(prefix_pages), prefix_pages.numel(), _lib.ptr(prefix_length))
-    return _attend("htn_shared_prefix_attention", q, key_pages, value_pages, prefix, page_table,
-                   query_starts, lengths, (), out)
+    return _attend("htn_shared_prefix_attention", q, key_pages, value_pages,
+                   (prefix_pages, prefix_length), page_table, query_starts, lengths, (), out)

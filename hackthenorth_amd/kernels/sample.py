@@ -6,13 +6,15 @@ equals, with weights exp(logit / temperature). Of them are kept, in turn: the fi
 top_k; the shortest leading part that holds top_p of the weight so far; those that
 weigh at least min_p times the largest. The answer is the first token whose
 cumulative weight passes `uniform` times the weight kept. Random numbers come from
-the caller, so a draw can be repeated, and weights are summed exactly (64-bit fixed
-point), so a row's token does not depend on the batch it is drawn in.
+the caller, so a draw can be repeated, and weights are summed as 64-bit integers, so
+a row's token does not depend on the batch it is drawn in.
 """
+import functools
+
 import torch
 
 from .. import _lib
-from .paged import _check_device, _on
+from .paged import _launch, _place
 
 
 def _setting(value, name, rows, dtype, low):
@@ -26,6 +28,11 @@ def _setting(value, name, rows, dtype, low):
     return None, value
 
 
+@functools.lru_cache(maxsize=256)
+def _scratch_bytes(rows, vocab):
+    return max(16, _lib.load().htn_sample_scratch_bytes(rows, vocab))
+
+
 def sample_token(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None):
     """One token per row of logits [..., V] (bf16 or fp32): int64 [...].
 
@@ -35,14 +42,15 @@ def sample_token(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0
     token. Logits of -inf and NaN are masked, tokens of +inf share all the weight;
     a row with nothing left gives -1. `out`, when given, receives the tokens.
     """
-    if logits.dim() < 1 or logits.dtype not in (torch.bfloat16, torch.float32) \
-            or 0 in logits.shape:
+    shape = logits.shape
+    if len(shape) < 1 or logits.dtype not in (torch.bfloat16, torch.float32) or 0 in shape:
         raise ValueError("sample_token expects bf16 or fp32 logits [..., V]")
-    vocab = logits.shape[-1]
-    flat = logits.reshape(-1, vocab)
-    if flat.stride(1) != 1 or (flat.shape[0] > 1 and flat.stride(0) < vocab):
+    vocab = shape[-1]
+    flat = logits if len(shape) == 2 else logits.reshape(-1, vocab)
+    rows, strides = flat.shape[0], flat.stride()
+    if strides[1] != 1 or (rows > 1 and strides[0] < vocab):
         flat = flat.contiguous()
-    rows = flat.shape[0]
+        strides = (vocab, 1)
     if uniform.dtype != torch.float32 or uniform.numel() != rows or not uniform.is_contiguous():
         raise ValueError("uniform must be contiguous float32 with one value per row")
     heat, heat_all = _setting(temperature, "temperature", rows, torch.float32, 0.0)
@@ -50,15 +58,13 @@ def sample_token(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0
     p, p_all = _setting(top_p, "top_p", rows, torch.float32, 0.0)
     m, m_all = _setting(min_p, "min_p", rows, torch.float32, 0.0)
     if out is None:
-        out = torch.empty(logits.shape[:-1], dtype=torch.int64, device=logits.device)
-    elif out.dtype != torch.int64 or out.shape != logits.shape[:-1] or not out.is_contiguous():
+        out = torch.empty(shape[:-1], dtype=torch.int64, device=logits.device)
+    elif out.dtype != torch.int64 or out.shape != shape[:-1] or not out.is_contiguous():
         raise ValueError("out must be contiguous int64 with one entry per row")
-    _check_device(flat, uniform, heat, k, p, m, out)
-    nbytes = _lib.load().htn_sample_scratch_bytes(rows, vocab)
-    scratch = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=flat.device)
-    with _on(flat.device):
-        _lib.call("htn_sample", _lib.ptr(flat), flat.stride(0), int(flat.dtype == torch.float32),
-                  rows, vocab, _lib.ptr(uniform), _lib.ptr(heat), float(heat_all), _lib.ptr(k),
-                  min(int(k_all), vocab), _lib.ptr(p), float(p_all), _lib.ptr(m), float(m_all),
-                  _lib.ptr(out), _lib.ptr(scratch), nbytes, _lib.stream(flat.device))
+    index = _place(flat, uniform, heat, k, p, m, out)
+    nbytes = _scratch_bytes(rows, vocab)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=flat.device)
+    _launch("htn_sample", index, flat.data_ptr(), strides[0], flat.dtype is torch.float32, rows,
+            vocab, uniform.data_ptr(), _lib.ptr(heat), heat_all, _lib.ptr(k), min(int(k_all), vocab),
+            _lib.ptr(p), p_all, _lib.ptr(m), m_all, out.data_ptr(), scratch.data_ptr(), nbytes)
     return out

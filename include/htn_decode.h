@@ -578,15 +578,15 @@ int htn_shared_prefix_attention(const void* q, int64_t q_st, int64_t q_sh, const
 /* ---------------------------------------------------------------- sampling
  *
  * out[r] = a token of row r (logits bf16, or fp32 with fp32 != 0; rows row_st
- * elements apart; vocab at most 2^19, rows at most 65535), drawn by uniform[r]
+ * elements apart; vocab at most 524160, rows at most 65535), drawn by uniform[r]
  * in [0, 1). A row's tokens are taken in order of falling logit, the lowest id
  * first among equals, with weights exp(logit / T). Kept are, in turn: the first
  * top_k of them (0 or less: all); of these the shortest leading part that holds
  * top_p of their weight (at least one token; 1 or more: all); of these the ones
  * that weigh at least min_p times the largest. The answer is the first token
  * whose cumulative weight passes uniform[r] times the weight kept. T not above
- * 0 gives the first token. Weights are summed in 64-bit fixed point (2^-44 of
- * the largest), so equal inputs give equal tokens in every batch. NaN and -inf
+ * 0 gives the first token. Weights are summed as integers (2^-34 of a token's
+ * weight at most is lost), so a row's token is the same in every batch. NaN and -inf
  * are masked, +inf tokens share all the weight; a row with nothing left gives
  * -1. Each setting is a device array with one value per row, or NULL and the
  * value after it for all rows. scratch: htn_sample_scratch_bytes bytes, no

@@ -1,9 +1,10 @@
 """sample_token against the definition in 64 bits, one row at a time.
 
-Tokens have to be equal. The kernel's weights are off by half of 2^-44 of the largest
-each, the reference's by 2^-53 relative, so the two part only where a border between
-two tokens falls within some 2^-36 of the point drawn: less than 1e-6 over all rows
-here, and the inputs are fixed by their seeds.
+Tokens have to be equal. The kernel's weights are off by 2^-34 relative each, the
+reference's by 2^-53, so a running sum of n tokens is off by some sqrt(n) 2^-34 of a
+weight where the next border is a whole weight away: a draw falls between with a
+probability of about 1e-8, less than 1e-4 over all rows here, and the inputs are
+fixed by their seeds.
 """
 import pytest
 import torch
