@@ -247,6 +247,42 @@ __device__ __forceinline__ float wave_max(float v) {
   return fmaxf(fmaxf(readlane(v, 0), readlane(v, 16)), fmaxf(readlane(v, 32), readlane(v, 48)));
 }
 
+// v plus that of the lanes that a DPP step brings (none: 0).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t add_dpp(uint32_t v) {
+  return v + __builtin_amdgcn_update_dpp(0u, v, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t add_dpp(uint64_t v) {
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0u, static_cast<uint32_t>(v), CTRL, ROWS, 0xf, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0u, static_cast<uint32_t>(v >> 32), CTRL, ROWS, 0xf, false);
+  return v + (static_cast<uint64_t>(hi) << 32 | lo);
+}
+
+// Running sums within each 16-lane row (row_shr 1, 2, 4, 8), and over the wave
+// (the rows' last lanes to the row behind, row 1's to the upper half). All 64 lanes
+// must be active.
+template <typename T>
+__device__ __forceinline__ T row_scan(T v) {
+  v = add_dpp<0x111, 0xf>(v);
+  v = add_dpp<0x112, 0xf>(v);
+  v = add_dpp<0x114, 0xf>(v);
+  return add_dpp<0x118, 0xf>(v);
+}
+template <typename T>
+__device__ __forceinline__ T wave_scan(T v) {
+  v = row_scan(v);
+  v = add_dpp<0x142, 0xa>(v);
+  return add_dpp<0x143, 0xc>(v);
+}
+
+// The last lane's value, wave-uniform.
+__device__ __forceinline__ uint32_t wave_last(uint32_t v) { return __builtin_amdgcn_readlane(v, 63); }
+__device__ __forceinline__ uint64_t wave_last(uint64_t v) {
+  return static_cast<uint64_t>(wave_last(static_cast<uint32_t>(v >> 32))) << 32 |
+         wave_last(static_cast<uint32_t>(v));
+}
+
 __device__ __forceinline__ uint64_t wave_max_u64(uint64_t v) {
 #pragma unroll
   for (int m = 32; m >= 1; m >>= 1) {

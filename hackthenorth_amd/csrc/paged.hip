@@ -145,7 +145,7 @@ __global__ __launch_bounds__(kBlock) void norm_rope_paged_kernel(AppendArgs a) {
 
 // ------------------------------------------------------------------ attention
 
-constexpr int kFewRows = 16;               // query rows of a block whose waves split the slots
+constexpr int kFewRows = 32;               // query rows of a block whose waves split the slots, at most
 constexpr int kManyRows = 128;             // and of one whose waves split the rows
 constexpr int kGroupBytes = 16 * D * 2;    // K or V of 16 slots
 constexpr int kTileBytes = 2 * kSplit * D * 2;
@@ -153,9 +153,9 @@ constexpr int kRing = 2;                   // staged 64-slot tiles
 
 struct PlanEntry {
   int part;     // first row of the sequence's partials
-  int chunks;   // parts that each row's slots are split in
+  int chunks;   // parts that each row's slots are split in; 0: its blocks finish their rows
   int stride;   // rows that a block's partials take
-  int pad;
+  int split;    // (first entry) whether any sequence is split
 };
 
 struct PagedArgs {
@@ -197,16 +197,6 @@ __device__ __forceinline__ Slots slots_of(int p_first, int p_last, int lo0, int 
   return s;
 }
 
-// One block's work.
-struct Item {
-  int seq;             // sequence, or -1 for the shared prefix
-  int t0, n, p0;       // its tokens
-  int tile, rows;      // row tile, and the rows in it
-  int kvh, chunk, chunks;
-  int part;            // first row of the block's partials, or -1: the block finishes its rows
-  int found;
-};
-
 struct SeqWork {
   Span span;
   int rows, tile_rows, row_tiles, max_tiles;
@@ -219,20 +209,22 @@ __device__ __forceinline__ int prefix_slots(const PagedArgs& a) {
 }
 
 // Sequence s of the plan: with a shared prefix, 0 is the prefix under all rows
-// and sequence j is s = j + 1.
-__device__ __forceinline__ SeqWork seq_work(const PagedArgs& a, int s, int prefix) {
+// and sequence j is s = j + 1. `bad` if the starts around it fall or leave the
+// batch.
+__device__ __forceinline__ SeqWork seq_work(const PagedArgs& a, int s, int prefix, bool& bad) {
   SeqWork w;
   const bool shared = a.prefix_length != nullptr;
   const int j = shared ? s - 1 : s;
   Slots all;
   if (j < 0) {
     const int64_t end = a.starts[a.B];
-    w.span.t0 = 0;
-    w.span.n = end < 0 ? 0 : (end > a.T ? a.T : static_cast<int>(end));
-    w.span.p0 = 0;
+    bad |= end < 0 || end > a.T;
+    w.span = Span{0, bad ? 0 : static_cast<int>(end), 0};
     all = slots_of(0, prefix - 1, 0, 0, 0);
   } else {
-    w.span = make_span(a.starts[j], a.starts[j + 1], a.lengths[j], a.T, a.table_pages << a.page_shift);
+    const int64_t s0 = a.starts[j], s1 = a.starts[j + 1];
+    bad |= s0 < 0 || s1 < s0 || s1 > a.T;
+    w.span = make_span(s0, s1, a.lengths[j], a.T, a.table_pages << a.page_shift);
     all = slots_of(0, w.span.p0 + w.span.n - 1, prefix, 0, 0);
   }
   w.rows = w.span.n * a.G;
@@ -251,99 +243,104 @@ __device__ __forceinline__ SeqWork seq_work(const PagedArgs& a, int s, int prefi
 // Tiles that a block takes at least, where a row's slots are split: a split
 // writes and merges a partial of its rows (520 bytes each) for K and V of 32 KB
 // a tile.
-constexpr int kMinTilesFew = 2, kMinTilesMany = 8;
+constexpr int kMinTiles = 2;
 
-__device__ __forceinline__ int chunks_of(const SeqWork& w, long per_block) {
-  const long least = w.tile_rows == kFewRows ? kMinTilesFew : kMinTilesMany;
-  const long c = per_block > least ? per_block : least;
-  const int n = static_cast<int>((w.max_tiles + c - 1) / c);
-  return n < 1 ? 1 : n;
+__device__ __forceinline__ int chunks_of(const SeqWork& w, uint32_t per_block) {
+  const uint32_t n = (w.max_tiles + per_block - 1) / per_block;
+  return n < 1 ? 1 : static_cast<int>(n);
 }
 
 __device__ __forceinline__ int part_stride(const SeqWork& w) {
   return w.rows < kManyRows ? (w.rows + 15) / 16 * 16 : kManyRows;
 }
 
-// Which rows, K/V head and slots this block takes. Every block derives the same
-// plan from starts and lengths: the tiles of all rows over `target` blocks give
-// the tiles per block, each sequence's rows are cut in equal chunks of at most
-// that many, and blocks are numbered sequence by sequence, in each by row tile
-// (the last, longest, first), chunk and K/V head. Blocks past the last have
-// nothing to do. A sequence's chunks number below twice its tiles over the
-// tiles per block where they are two or more, so all split blocks number below
-// 2 target, and all blocks at most target plus one per (row tile, K/V head).
-__device__ __forceinline__ void make_plan(const PagedArgs& a, Item* item, uint64_t* red) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int prefix = prefix_slots(a);
+// One block's work.
+struct Item {
+  int seq;             // sequence, or -1 for the shared prefix
+  int t0, n, p0;       // its tokens
+  int tile, rows;      // row tile, and the rows in it
+  int kvh, chunk, chunks;
+  int part;            // first row of the block's partials, or -1: the block finishes its rows
+};
+
+// Which rows, K/V head and slots this block takes; false if none. Every wave
+// derives the same plan from starts and lengths, a sequence a lane: the tiles of
+// all rows over `target` blocks give the tiles per block, each sequence's rows are
+// cut in equal chunks of at most that many, and blocks are numbered sequence by
+// sequence, in each by row tile (the last, longest, first), chunk and K/V head.
+//
+// A sequence's chunks number below twice its tiles over the tiles per block where
+// they are two or more, so all split blocks number below 2 target, and all blocks
+// at most target plus one per (row tile, K/V head). With 64 sequences or fewer the
+// tiles per block are raised until all blocks fit `target` (they run at once).
+__device__ __forceinline__ bool make_plan(const PagedArgs& a, int prefix, Item& it) {
+  const int lane = threadIdx.x & 63;
   const bool shared = a.prefix_length != nullptr;
   const int n = a.B + (shared ? 1 : 0);
   uint64_t total = 0;
+  int items = 0;
   SeqWork w{};
   bool bad = false;
-  for (int s = tid; s < n; s += kBlock) {
-    w = seq_work(a, s, prefix);
+  for (int s = lane; s < n; s += kWave) {
+    w = seq_work(a, s, prefix, bad);
     total += static_cast<uint64_t>(w.row_tiles) * w.max_tiles * a.Hkv;
-    const int j = shared && s > 0 ? s - 1 : s;
-    bad |= j < a.B && a.starts[j + 1] < a.starts[j];
+    items += w.row_tiles * a.Hkv;
   }
   // Starts must rise: the bounds of the blocks and partials count every row once.
-  bad |= a.starts[0] < 0 || a.starts[a.B] > a.T;
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) total += __shfl_xor(total, m, kWave);
-  if (lane == 0) red[wave] = total;
-  if (tid == 0) item->found = 0;
-  bad = __syncthreads_or(bad);
-  total = (red[0] + red[1]) + (red[2] + red[3]);
-  const long per_block = static_cast<long>((total + a.target - 1) / a.target);
+  if (__any(bad)) {
+    if (blockIdx.x == 0)
+      for (int s = threadIdx.x; s < n; s += kBlock) a.plan[s] = PlanEntry{0, 0, 0, 0};
+    return false;
+  }
+  total = wave_last(wave_scan(total));
+  items = wave_last(wave_scan(static_cast<uint32_t>(items)));
+  uint32_t per_block = static_cast<uint32_t>((total + a.target - 1) / a.target);
+  per_block = per_block > kMinTiles ? per_block : kMinTiles;
+  if (n <= kWave && items <= a.target)
+    for (;; per_block += 1 + per_block / 16) {
+      const uint32_t mine = lane < n ? w.row_tiles * chunks_of(w, per_block) * a.Hkv : 0;
+      if (wave_last(wave_scan(mine)) <= static_cast<uint32_t>(a.target)) break;
+    }
   // Blocks (low half) and rows of partials (high half) before each sequence.
   uint64_t base = 0;
-  for (int s0 = 0; s0 < n; s0 += kBlock) {
-    const int s = s0 + tid;
-    if (n > kBlock) w = seq_work(a, s < n ? s : n - 1, prefix);
+  bool found = false;
+  for (int s0 = 0; s0 < n; s0 += kWave) {
+    const int s = s0 + lane;
+    if (n > kWave) w = seq_work(a, s < n ? s : n - 1, prefix, bad);
     const int chunks = s < n ? chunks_of(w, per_block) : 0;
-    const int blocks = s < n && !bad ? w.row_tiles * chunks * a.Hkv : 0;
-    const bool split = !bad && (shared || chunks > 1);
+    const int blocks = w.row_tiles * chunks * a.Hkv;
+    const bool split = blocks && (shared || chunks > 1);
     const int stride = part_stride(w);
-    uint64_t mine = static_cast<uint64_t>(blocks) |
-                    (split ? static_cast<uint64_t>(blocks) * stride << 32 : 0);
-    uint64_t sum = mine;
-#pragma unroll
-    for (int m = 1; m < kWave; m <<= 1) {
-      const uint64_t o = __shfl_up(sum, m, kWave);
-      if (lane >= m) sum += o;
-    }
-    __syncthreads();
-    if (lane == 63) red[wave] = sum;
-    __syncthreads();
-    uint64_t before = base;
-#pragma unroll
-    for (int v = 0; v < kBlock / kWave; ++v) {
-      if (v < wave) before += red[v];
-      base += red[v];
-    }
-    const uint64_t first = before + sum - mine;
+    const uint64_t mine = static_cast<uint64_t>(blocks) |
+                          (split ? static_cast<uint64_t>(blocks) * stride << 32 : 0);
+    const uint64_t sum = wave_scan(mine);
+    const uint64_t first = base + sum - mine;
+    base += wave_last(sum);
     const int at = static_cast<int>(blockIdx.x) - static_cast<int>(first & 0xffffffffu);
     const int part = static_cast<int>(first >> 32);
-    if (blockIdx.x == 0 && s < n) a.plan[s] = PlanEntry{part, split ? chunks : 0, stride, 0};
-    if (at >= 0 && at < blocks) {
-      Item it;
-      it.seq = shared ? s - 1 : s;
-      it.t0 = w.span.t0;
-      it.n = w.span.n;
-      it.p0 = w.span.p0;
-      it.kvh = at % a.Hkv;
-      const int rest = at / a.Hkv;
-      it.chunk = rest % chunks;
-      it.chunks = chunks;
-      it.tile = w.row_tiles - 1 - rest / chunks;
-      const int left = w.rows - it.tile * w.tile_rows;
-      it.rows = left < w.tile_rows ? left : w.tile_rows;
-      it.part = split ? part + ((it.tile * chunks + it.chunk) * a.Hkv + it.kvh) * stride : -1;
-      it.found = 1;
-      *item = it;
-    }
+    if (blockIdx.x == 0 && threadIdx.x < kWave && s < n) a.plan[s] = PlanEntry{part, split ? chunks : 0, stride, 0};
+    const uint64_t mask = __ballot(at >= 0 && at < blocks);
+    if (!mask) continue;
+    found = true;
+    const int src = __builtin_ctzll(mask);
+    auto of = [&](int v) { return __builtin_amdgcn_readlane(v, src); };
+    it.seq = s0 + src - (shared ? 1 : 0);
+    it.t0 = of(w.span.t0);
+    it.n = of(w.span.n);
+    it.p0 = of(w.span.p0);
+    it.chunks = of(chunks);
+    const int place = of(at), tile_rows = of(w.tile_rows);
+    it.kvh = place % a.Hkv;
+    const int rest = place / a.Hkv;
+    it.chunk = rest % it.chunks;
+    it.tile = of(w.row_tiles) - 1 - rest / it.chunks;
+    const int left = of(w.rows) - it.tile * tile_rows;
+    it.rows = left < tile_rows ? left : tile_rows;
+    it.part = of(split) ? of(part) + ((it.tile * it.chunks + it.chunk) * a.Hkv + it.kvh) * of(stride) : -1;
+    if (blockIdx.x) break;
   }
-  __syncthreads();
+  if (blockIdx.x == 0 && threadIdx.x == 0) a.plan[0].split = base >> 32 ? 1 : 0;
+  return found;
 }
 
 // Where a 16-slot group's K or V rows lie in a pool: an element offset, and the
@@ -450,33 +447,40 @@ __device__ __forceinline__ void row_of(const PagedArgs& a, const Item& it, int t
   h = it.kvh * a.G + rr % a.G;
 }
 
-// Up to 16 query rows (one token of a sequence, or a few): the four waves split
+// Up to 32 query rows (one token of a sequence, or a few): the four waves split
 // the slots, 16 of each tile, and each runs a softmax of its own over them; the
 // states meet in LDS at the end. Slots are the M index of S^T = K Q^T and query
-// rows the N index; the scores' layout is the P^T operand's of O^T += V^T P^T,
-// whose K = 32 holds the 16 slots twice, with the upper and with the lower bf16
-// half of their weights (about 16 bits; the product waits for memory anyway).
-// An infinite V in a slot that every row sees gives NaN (the lower half is 0).
+// rows the N index (NT tiles of 16); the scores' layout is the P^T operand's of
+// O^T += V^T P^T, whose K = 32 holds the 16 slots twice, with the upper and with
+// the lower bf16 half of their weights (about 16 bits; the product waits for
+// memory anyway). An infinite V in a slot that every row sees gives NaN (the lower
+// half is 0).
+template <int NT>
 __device__ __forceinline__ void attend_few(const PagedArgs& a, const Item& it, const Slots& sl,
                                            const int32_t* table, const int* rowpos,
-                                           unsigned char* ring, float (&wm)[4][kFewRows],
-                                           float (&wl)[4][kFewRows]) {
+                                           unsigned char* ring, float (&wm)[4][16], float (&wl)[4][16]) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, quad = lane >> 4;
   const int i0 = static_cast<int>(static_cast<long>(sl.tiles) * it.chunk / it.chunks);
   const int i1 = static_cast<int>(static_cast<long>(sl.tiles) * (it.chunk + 1) / it.chunks);
-  int t, h;
-  row_of(a, it, kFewRows, col < it.rows ? col : 0, t, h);
-  u32x4 qf[4];
-  const bf16_t* qrow = a.q + t * a.q_st + h * a.q_sh + 8 * quad;
-#pragma unroll
-  for (int ks = 0; ks < 4; ++ks) qf[ks] = *reinterpret_cast<const u32x4*>(qrow + 32 * ks);
-  const int pos = it.seq < 0 ? rowpos[t - it.t0 - it.tile * kFewRows / a.G] : it.p0 + (t - it.t0);
-  const Sight sight = sight_of(pos, sl, a.window);
   const int sinks = a.window ? a.sinks : 0;
-  const int all_hi = min16(sight.vhi), all_lo = -min16(-sight.vlo);  // padding columns repeat row 0
-
+  u32x4 qf[NT][4];
+  Sight sight[NT];
+  int all_hi = 0x7fffffff, all_lo = -0x7fffffff;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int r = 16 * n + col;
+    int t, h;
+    row_of(a, it, kFewRows, r < it.rows ? r : 0, t, h);  // padding columns repeat row 0
+    const bf16_t* qrow = a.q + t * a.q_st + h * a.q_sh + 8 * quad;
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) qf[n][ks] = *reinterpret_cast<const u32x4*>(qrow + 32 * ks);
+    sight[n] = sight_of(it.seq < 0 ? rowpos[t] : it.p0 + (t - it.t0), sl, a.window);
+    const int lo = min16(sight[n].vhi), hi = -min16(-sight[n].vlo);
+    all_hi = lo < all_hi ? lo : all_hi;
+    all_lo = hi > all_lo ? hi : all_lo;
+  }
   uint32_t kvoff[4], vvoff[4];
 #pragma unroll
   for (int u = 0; u < 4; ++u) {
@@ -512,10 +516,15 @@ __device__ __forceinline__ void attend_few(const PagedArgs& a, const Item& it, c
     vaddr[j] = base + kGroupBytes +
                static_cast<uint32_t>(vr * 256 + (((2 * j + ((col & 3) >> 1) + 2 * (vr & 7)) & 15) * 16) +
                                      (col & 1) * 8);
-  f32x4_t acc[8];
+  f32x4_t acc[NT][8];
+  float m[NT], l[NT];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) acc[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, l = 0.f;
+  for (int n = 0; n < NT; ++n) {
+    m[n] = -INFINITY;
+    l[n] = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[n][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
   for (int i = i0; i < i1; ++i) {
     const uint32_t ro = static_cast<uint32_t>((i - i0) % kRing) * kTileBytes;
     u32x4 k[4];
@@ -550,80 +559,84 @@ __device__ __forceinline__ void attend_few(const PagedArgs& a, const Item& it, c
     // its V is to be read once more.
     const bool late = __any(odd);
     if (!late) stage(i + kRing);
-    f32x4_t st = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) st = mfma(k[ks], qf[ks], st);
-    float sc[4];
-    if (whole) {
+    for (int n = 0; n < NT; ++n) {
+      f32x4_t st = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int r = 0; r < 4; ++r) sc[r] = st[r] * a.scale2;
-    } else {
+      for (int ks = 0; ks < 4; ++ks) st = mfma(k[ks], qf[n][ks], st);
+      float sc[4];
+      if (whole) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int s = slot + r;
-        sc[r] = s <= sight.vhi && (s >= sight.vlo || s < sinks) ? st[r] * a.scale2 : -INFINITY;
+        for (int r = 0; r < 4; ++r) sc[r] = st[r] * a.scale2;
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int s = slot + r;
+          sc[r] = s <= sight[n].vhi && (s >= sight[n].vlo || s < sinks) ? st[r] * a.scale2 : -INFINITY;
+        }
       }
-    }
-    const float tmax = quad_max(fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])));
-    const float m_new = fmaxf(m, tmax);
-    const float ms = m_new == -INFINITY ? 0.f : m_new;  // nothing visible yet: weights of 0
-    if (!__all(m_new == m)) {
-      const float alpha = __builtin_amdgcn_exp2f(m - ms);
-      l *= alpha;
+      const float tmax = quad_max(fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])));
+      const float m_new = fmaxf(m[n], tmax);
+      const float ms = m_new == -INFINITY ? 0.f : m_new;  // nothing visible yet: weights of 0
+      if (!__all(m_new == m[n])) {
+        const float alpha = __builtin_amdgcn_exp2f(m[n] - ms);
+        l[n] *= alpha;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) acc[j] *= alpha;
-    }
-    m = m_new;
-    float p[4];
+        for (int j = 0; j < 8; ++j) acc[n][j] *= alpha;
+      }
+      m[n] = m_new;
+      float p[4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) p[r] = __builtin_amdgcn_exp2f(sc[r] - ms);
-    l += (p[0] + p[1]) + (p[2] + p[3]);
-    const uint32_t h0 = pack_bf2(p[0], p[1]), h1 = pack_bf2(p[2], p[3]);
-    const u32x4 ph = {h0, h1, pack_bf2(p[0] - bf_lo(h0), p[1] - bf_hi(h0)),
-                      pack_bf2(p[2] - bf_lo(h1), p[3] - bf_hi(h1))};
+      for (int r = 0; r < 4; ++r) p[r] = __builtin_amdgcn_exp2f(sc[r] - ms);
+      l[n] += (p[0] + p[1]) + (p[2] + p[3]);
+      const uint32_t h0 = pack_bf2(p[0], p[1]), h1 = pack_bf2(p[2], p[3]);
+      const u32x4 ph = {h0, h1, pack_bf2(p[0] - bf_lo(h0), p[1] - bf_hi(h0)),
+                        pack_bf2(p[2] - bf_lo(h1), p[3] - bf_hi(h1))};
 #pragma unroll
-    for (int j = 0; j < 8; ++j) acc[j] = mfma(u32x4{v[j].x, v[j].y, v[j].x, v[j].y}, ph, acc[j]);
-    if (late) {
-      add_nonfinite(lds + ro + kGroupBytes, 16, s0, sight, sinks, quad, acc);
-      stage(i + kRing);
+      for (int j = 0; j < 8; ++j) acc[n][j] = mfma(u32x4{v[j].x, v[j].y, v[j].x, v[j].y}, ph, acc[n][j]);
+      if (late) add_nonfinite(lds + ro + kGroupBytes, 16, s0, sight[n], sinks, quad, acc[n]);
     }
+    if (late) stage(i + kRing);
   }
   // The waves' states, in LDS rows of 132 floats (the 16 rows in other banks).
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  l = quad_sum(l);
-  __syncthreads();
   float* wacc = reinterpret_cast<float*>(ring);
   constexpr int kRowFloats = D + 4;
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
-    *reinterpret_cast<f32x4_t*>(wacc + (wave * kFewRows + col) * kRowFloats + 16 * j + 4 * quad) = acc[j];
-  if (quad == 0) {
-    wm[wave][col] = m;
-    wl[wave][col] = l;
-  }
-  __syncthreads();
-  for (int r = wave; r < it.rows; r += 4) {
-    const float M = fmaxf(fmaxf(wm[0][r], wm[1][r]), fmaxf(wm[2][r], wm[3][r]));
-    float L = 0.f, x = 0.f, y = 0.f;
-    if (M != -INFINITY) {
+  for (int n = 0; n < NT; ++n) {
+    l[n] = quad_sum(l[n]);
+    __syncthreads();
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const float f = __builtin_amdgcn_exp2f(wm[w][r] - M);
-        const float2 o = *reinterpret_cast<const float2*>(wacc + (w * kFewRows + r) * kRowFloats + 2 * lane);
-        L = fmaf(f, wl[w][r], L);
-        x = fmaf(f, o.x, x);
-        y = fmaf(f, o.y, y);
-      }
+    for (int j = 0; j < 8; ++j)
+      *reinterpret_cast<f32x4_t*>(wacc + (wave * 16 + col) * kRowFloats + 16 * j + 4 * quad) = acc[n][j];
+    if (quad == 0) {
+      wm[wave][col] = m[n];
+      wl[wave][col] = l[n];
     }
-    if (it.part >= 0) {
-      const long row = it.part + r;
-      *reinterpret_cast<float2*>(a.part + row * D + 2 * lane) = make_float2(x, y);
-      if (lane == 0) a.ml[row] = make_float2(M, L);
-    } else {
-      int tr, hr;
-      row_of(a, it, kFewRows, r, tr, hr);
-      const float inv = M == -INFINITY ? 0.f : 1.0f / L;
-      *reinterpret_cast<uint32_t*>(a.out + tr * a.o_st + hr * a.o_sh + 2 * lane) = pack_bf2(x * inv, y * inv);
+    __syncthreads();
+    for (int c = wave; c < 16 && 16 * n + c < it.rows; c += 4) {
+      const float M = fmaxf(fmaxf(wm[0][c], wm[1][c]), fmaxf(wm[2][c], wm[3][c]));
+      float L = 0.f, x = 0.f, y = 0.f;
+      if (M != -INFINITY) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const float f = __builtin_amdgcn_exp2f(wm[w][c] - M);
+          const float2 o = *reinterpret_cast<const float2*>(wacc + (w * 16 + c) * kRowFloats + 2 * lane);
+          L = fmaf(f, wl[w][c], L);
+          x = fmaf(f, o.x, x);
+          y = fmaf(f, o.y, y);
+        }
+      }
+      if (it.part >= 0) {
+        const long row = it.part + 16 * n + c;
+        *reinterpret_cast<float2*>(a.part + row * D + 2 * lane) = make_float2(x, y);
+        if (lane == 0) a.ml[row] = make_float2(M, L);
+      } else {
+        int tr, hr;
+        row_of(a, it, kFewRows, 16 * n + c, tr, hr);
+        const float inv = M == -INFINITY ? 0.f : 1.0f / L;
+        *reinterpret_cast<uint32_t*>(a.out + tr * a.o_st + hr * a.o_sh + 2 * lane) = pack_bf2(x * inv, y * inv);
+      }
     }
   }
 }
@@ -837,28 +850,15 @@ __device__ __forceinline__ void attend_many(const PagedArgs& a, const Item& it, 
 
 __global__ __launch_bounds__(kBlock, 2) void paged_attention_kernel(PagedArgs a) {
   extern __shared__ __align__(16) unsigned char ring[];  // two staged tiles
-  __shared__ Item item;
-  __shared__ uint64_t red[4];
   __shared__ int rowpos[kManyRows];
-  __shared__ float wm[4][kFewRows], wl[4][kFewRows];
-  make_plan(a, &item, red);
-  if (!__builtin_amdgcn_readfirstlane(item.found)) return;
-  Item it;
-  it.seq = __builtin_amdgcn_readfirstlane(item.seq);
-  it.t0 = __builtin_amdgcn_readfirstlane(item.t0);
-  it.n = __builtin_amdgcn_readfirstlane(item.n);
-  it.p0 = __builtin_amdgcn_readfirstlane(item.p0);
-  it.tile = __builtin_amdgcn_readfirstlane(item.tile);
-  it.rows = __builtin_amdgcn_readfirstlane(item.rows);
-  it.kvh = __builtin_amdgcn_readfirstlane(item.kvh);
-  it.chunk = __builtin_amdgcn_readfirstlane(item.chunk);
-  it.chunks = __builtin_amdgcn_readfirstlane(item.chunks);
-  it.part = __builtin_amdgcn_readfirstlane(item.part);
+  __shared__ float wm[4][16], wl[4][16];
+  const int prefix = __builtin_amdgcn_readfirstlane(prefix_slots(a));
+  Item it{};
+  if (!make_plan(a, prefix, it)) return;
   const bool few = it.n * a.G <= kFewRows;
   const int tile_rows = few ? kFewRows : kManyRows;
   // The tile's first and last token, and the slots that its rows see.
   const int first = it.tile * tile_rows / a.G, last = (it.tile * tile_rows + it.rows - 1) / a.G;
-  const int prefix = __builtin_amdgcn_readfirstlane(prefix_slots(a));
   Slots sl;
   const int32_t* table;
   if (it.seq < 0) {
@@ -877,72 +877,80 @@ __global__ __launch_bounds__(kBlock, 2) void paged_attention_kernel(PagedArgs a)
     sl = slots_of(it.p0 + first, it.p0 + last, prefix, a.window, a.sinks);
     table = a.table + it.seq * a.table_st;
   }
-  if (few) attend_few(a, it, sl, table, rowpos, ring, wm, wl);
+  if (it.rows <= 16 && few) attend_few<1>(a, it, sl, table, rowpos, ring, wm, wl);
+  else if (few) attend_few<2>(a, it, sl, table, rowpos, ring, wm, wl);
   else attend_many(a, it, sl, table, rowpos, ring);
 }
 
 // The rows whose slots were split, one wave each:
 //   out = sum_c 2^(m_c - M) acc_c / sum_c 2^(m_c - M) l_c,  M = max_c m_c
 // over the chunks of the row's own slots and, where one is shared, of the prefix.
+// A lane first holds a chunk's (m, l); then each half of the wave takes every
+// other chunk's row, four dims a lane, eight chunks' loads in flight.
 __global__ __launch_bounds__(kBlock) void paged_merge_kernel(PagedArgs a) {
-  const int lane = threadIdx.x & 63;
-  const long orow = static_cast<long>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  const int t = static_cast<int>(orow / a.Hq), h = static_cast<int>(orow % a.Hq);
-  if (t >= a.T) return;
-  const int j = sequence_of(a.starts, a.B, t, lane);
-  if (j >= a.B) return;
+  const int lane = threadIdx.x & 63, half = lane >> 5, dim = 4 * (lane & 31);
+  if (!a.plan[0].split) return;
   const bool shared = a.prefix_length != nullptr;
-  const PlanEntry own = a.plan[j + (shared ? 1 : 0)];
-  if (!own.chunks) return;
-  const Span s = make_span(a.starts[j], a.starts[j + 1], a.lengths[j], a.T, a.table_pages << a.page_shift);
-  if (t < s.t0 || t >= s.t0 + s.n) return;
-  const int kvh = h / a.G;
-  float M = -INFINITY, L = 0.f, x = 0.f, y = 0.f;
-  auto fold = [&](const PlanEntry& p, int token, int tokens) {
-    const int r = token * a.G + h % a.G;
-    const int tile_rows = tokens * a.G <= kFewRows ? kFewRows : kManyRows;
-    const int tile = r / tile_rows;
-    long row = p.part + (static_cast<long>(tile) * p.chunks * a.Hkv + kvh) * p.stride + r % tile_rows;
-    const long step = static_cast<long>(a.Hkv) * p.stride;
-    constexpr int U = 4;
-    for (int c = 0; c < p.chunks; c += U) {
-      float2 o[U], ml[U];
+  const long rows = static_cast<long>(a.T) * a.Hq;
+  for (long orow = static_cast<long>(blockIdx.x) * 4 + (threadIdx.x >> 6); orow < rows;
+       orow += static_cast<long>(gridDim.x) * 4) {
+    const int t = static_cast<int>(orow / a.Hq), h = static_cast<int>(orow % a.Hq);
+    const int j = sequence_of(a.starts, a.B, t, lane);
+    if (j >= a.B) continue;
+    const PlanEntry own = a.plan[j + (shared ? 1 : 0)];
+    if (!own.chunks) continue;
+    const Span s = make_span(a.starts[j], a.starts[j + 1], a.lengths[j], a.T, a.table_pages << a.page_shift);
+    if (t < s.t0 || t >= s.t0 + s.n) continue;
+    const int kvh = h / a.G;
+    float M = -INFINITY, L = 0.f;
+    f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+    auto fold = [&](const PlanEntry& p, int token, int tokens) {
+      const int r = token * a.G + h % a.G;
+      const int tile_rows = tokens * a.G <= kFewRows ? kFewRows : kManyRows;
+      const long row = p.part + (static_cast<long>(r / tile_rows) * p.chunks * a.Hkv + kvh) * p.stride + r % tile_rows;
+      const long step = static_cast<long>(a.Hkv) * p.stride;
+      for (int c0 = 0; c0 < p.chunks; c0 += kWave) {
+        const int n = p.chunks - c0 < kWave ? p.chunks - c0 : kWave;
+        const float2 ml = lane < n ? a.ml[row + (c0 + lane) * step] : make_float2(-INFINITY, 0.f);
+        const float mb = fmaxf(M, wave_max(ml.x));
+        if (mb == -INFINITY) continue;
+        const float f0 = __builtin_amdgcn_exp2f(M - mb);
+        const float f = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - mb);
+        M = mb;
+        L = fmaf(L, f0, wave_sum(f * ml.y));
+        o *= f0;
+        constexpr int U = 8;
+        for (int c = 0; c < n; c += 2 * U) {
+          f32x4_t x[U];
+          float g[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const long rw = row + (c + u < p.chunks ? u : 0) * step;
-        o[u] = *reinterpret_cast<const float2*>(a.part + rw * D + 2 * lane);
-        ml[u] = a.ml[rw];
-        if (c + u >= p.chunks) ml[u].x = -INFINITY;
+          for (int u = 0; u < U; ++u) {
+            const int at = c + 2 * u + half, k = at < n ? at : 0;
+            x[u] = *reinterpret_cast<const f32x4_t*>(a.part + (row + (c0 + k) * step) * D + dim);
+            const float fk = __shfl(f, k, kWave);
+            g[u] = at < n ? fk : 0.f;
+          }
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+            if (g[u] != 0.f) o += x[u] * g[u];  // a chunk that saw nothing wrote no weights
+        }
       }
-      row += U * step;
-      float mb = M;
+    };
+    fold(own, t - s.t0, s.n);
+    if (shared) fold(a.plan[0], t, static_cast<int>(a.starts[a.B]));
 #pragma unroll
-      for (int u = 0; u < U; ++u) mb = fmaxf(mb, ml[u].x);
-      if (mb == -INFINITY) continue;
-      const float f0 = __builtin_amdgcn_exp2f(M - mb);
-      x *= f0;
-      y *= f0;
-      L *= f0;
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (ml[u].x == -INFINITY) continue;
-        const float f = __builtin_amdgcn_exp2f(ml[u].x - mb);
-        x = fmaf(f, o[u].x, x);
-        y = fmaf(f, o[u].y, y);
-        L = fmaf(f, ml[u].y, L);
-      }
-      M = mb;
-    }
-  };
-  fold(own, t - s.t0, s.n);
-  if (shared) fold(a.plan[0], t, static_cast<int>(a.starts[a.B]));
-  const float inv = M == -INFINITY ? 0.f : 1.0f / L;
-  *reinterpret_cast<uint32_t*>(a.out + t * a.o_st + h * a.o_sh + 2 * lane) = pack_bf2(x * inv, y * inv);
+    for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], 32, kWave);
+    const float inv = M == -INFINITY ? 0.f : 1.0f / L;
+    if (half == 0)
+      *reinterpret_cast<uint2*>(a.out + t * a.o_st + h * a.o_sh + dim) =
+          make_uint2(pack_bf2(o[0] * inv, o[1] * inv), pack_bf2(o[2] * inv, o[3] * inv));
+  }
 }
 
 // ------------------------------------------------------------------ host
 
 constexpr int kTargetBlocks = 512;  // two per CU
+constexpr long kMergeBlocks = 2048;
 constexpr long kMaxSlots = 1L << 29;
 
 int page_shift_of(int64_t page) {
@@ -960,7 +968,7 @@ struct Sizes {
 Sizes sizes_of(long tokens, long batch, long q_heads, long kv_heads, bool shared) {
   Sizes s;
   const long rows = tokens * (q_heads / kv_heads), with = batch < tokens ? batch : tokens;
-  const long top = rows <= kFewRows ? kFewRows : (rows < kManyRows ? (rows + 15) / 16 * 16 : kManyRows);
+  const long top = rows < kManyRows ? (rows + 15) / 16 * 16 : kManyRows;
   s.plan = ((batch + 1) * static_cast<long>(sizeof(PlanEntry)) + 255) / 256 * 256;
   s.rows = 2L * kTargetBlocks * top;
   long tiles = rows / kManyRows + with;
@@ -990,13 +998,12 @@ int attend(PagedArgs& a, void* scratch, int64_t scratch_bytes, hipStream_t st) {
   a.scale2 = 1.4426950408889634f / sqrtf(static_cast<float>(D));
   constexpr int lds = kRing * kTileBytes;
   const long merge = (static_cast<long>(a.T) * a.Hq + 3) / 4;
-  if (merge >= (1L << 31)) return HTN_EUNSUPPORTED;
   static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_attention_kernel),
                                               hipFuncAttributeMaxDynamicSharedMemorySize, lds);
   (void)attr;  // a refused size surfaces as a launch error
   hipLaunchKernelGGL(paged_attention_kernel, dim3(static_cast<unsigned>(s.blocks)), dim3(kBlock), lds, st, a);
   if (launch_status() != HTN_OK) return HTN_ELAUNCH;
-  hipLaunchKernelGGL(paged_merge_kernel, dim3(static_cast<unsigned>(merge)), dim3(kBlock), 0, st, a);
+  hipLaunchKernelGGL(paged_merge_kernel, dim3(static_cast<unsigned>(merge < kMergeBlocks ? merge : kMergeBlocks)), dim3(kBlock), 0, st, a);
   return launch_status();
 }
 
