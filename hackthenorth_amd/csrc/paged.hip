@@ -439,6 +439,23 @@ __device__ __forceinline__ f32x4_t mfma(u32x4 x, u32x4 y, f32x4_t c) {
                                                  __builtin_bit_cast(bf16x8_t, y), c, 0, 0, 0);
 }
 
+// The largest of three; fmaxf first quiets each operand, an instruction of its own.
+// The compiler does not see the instruction: scores pass `settle` before.
+__device__ __forceinline__ float max3(float x, float y, float z) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));
+  return r;
+}
+
+// The wait states that a vector instruction must keep from the matrix instruction
+// whose result it reads (19 at most), which the compiler does not insert ahead of
+// inline asm.
+__device__ __forceinline__ void settle(f32x4_t (&s)[2][4]) {
+  asm volatile("s_nop 15\n\ts_nop 7"
+               : "+v"(s[0][0]), "+v"(s[0][1]), "+v"(s[0][2]), "+v"(s[0][3]), "+v"(s[1][0]), "+v"(s[1][1]),
+                 "+v"(s[1][2]), "+v"(s[1][3]));
+}
+
 // Token and head of row r of an item's row tile.
 __device__ __forceinline__ void row_of(const PagedArgs& a, const Item& it, int tile_rows, int r, int& t,
                                        int& h) {
@@ -648,7 +665,7 @@ __device__ __forceinline__ void attend_few(const PagedArgs& a, const Item& it, c
 // row's weights add up to 1.
 __device__ __forceinline__ void attend_many(const PagedArgs& a, const Item& it, const Slots& sl,
                                             const int32_t* table, const int* rowpos,
-                                            unsigned char* ring) {
+                                            unsigned char* ring, int2* bounds, int* odd_tile) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, quad = lane >> 4;
@@ -738,6 +755,7 @@ __device__ __forceinline__ void attend_many(const PagedArgs& a, const Item& it, 
     u32x2_t vw[2][8];
     issue_vt_tr<0>(va, vw[0]);
     issue_vt_tr<4096>(va, vw[1]);
+    settle(st);
     uint2 pb[2][4];
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
@@ -750,15 +768,16 @@ __device__ __forceinline__ void attend_many(const PagedArgs& a, const Item& it, 
             st[n][mt][r] = s <= sight[n].vhi && (s >= sight[n].vlo || s < sinks) ? st[n][mt][r] : -INFINITY;
           }
       }
-      float tmax = -INFINITY;
+      float tmax = max3(st[n][0][0], st[n][0][1], st[n][0][2]);
 #pragma unroll
-      for (int mt = 0; mt < 4; ++mt)
-        tmax = fmaxf(fmaxf(tmax, fmaxf(st[n][mt][0], st[n][mt][1])), fmaxf(st[n][mt][2], st[n][mt][3]));
-      tmax = quad_max(tmax);
+      for (int i = 3; i < 15; i += 2)
+        tmax = max3(tmax, st[n][i / 4][i % 4], st[n][(i + 1) / 4][(i + 1) % 4]);
+      tmax = quad_max(fmaxf(tmax, st[n][3][3]));
       const float m_new = fmaxf(m[n], tmax);
       const float ms = m_new == -INFINITY ? 0.f : m_new * a.scale2;
       if (!__all(m_new == m[n])) {
-        const float alpha = __builtin_amdgcn_exp2f(fmaf(m[n], a.scale2, -ms));
+        // Not 0, so that an infinity that was added stays one.
+        const float alpha = fmaxf(__builtin_amdgcn_exp2f(fmaf(m[n], a.scale2, -ms)), 1.2e-38f);
         sum[n] *= alpha;
 #pragma unroll
         for (int j = 0; j < 8; ++j) acc[n][j] *= alpha;
@@ -772,7 +791,6 @@ __device__ __forceinline__ void attend_many(const PagedArgs& a, const Item& it, 
         pb[n][mt] = make_uint2(pack_bf2(p[0], p[1]), pack_bf2(p[2], p[3]));
       }
     }
-    bool odd = false;
     auto weigh = [&](const u32x2_t (&v)[2][8], int mt) {
       u32x4 p[2];
 #pragma unroll
@@ -782,11 +800,7 @@ __device__ __forceinline__ void attend_many(const PagedArgs& a, const Item& it, 
       }
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        u32x4 x = {v[0][j].x, v[0][j].y, v[1][j].x, v[1][j].y};
-        if (!whole) {
-#pragma unroll
-          for (int r = 0; r < 4; ++r) x[r] = finite_pair(x[r], odd);
-        }
+        const u32x4 x = {v[0][j].x, v[0][j].y, v[1][j].x, v[1][j].y};
 #pragma unroll
         for (int n = 0; n < 2; ++n) acc[n][j] = mfma(x, p[n], acc[n][j]);
       }
@@ -800,28 +814,64 @@ __device__ __forceinline__ void attend_many(const PagedArgs& a, const Item& it, 
     __builtin_amdgcn_sched_barrier(0);
     wait_v16(vx);
     weigh(vx, 2);
-    if (__builtin_expect(__any(odd), 0)) {
-#pragma unroll 1
-      for (int g = 0; g < 4; ++g)
+  };
+  // The slots that all rows of the block see.
+  if (lane == 0) bounds[wave] = make_int2(all_hi, all_lo);
+  if (tid == 0) *odd_tile = 0;
+  lds_barrier();
+  int block_hi = bounds[0].x, block_lo = bounds[0].y;
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
-          add_nonfinite(ring + tb + kSplit * D * 2 + g * kGroupBytes, 16, s0 + 16 * g, sight[n], sinks, quad,
-                        acc[n]);
-    }
+  for (int w = 1; w < 4; ++w) {
+    block_hi = bounds[w].x < block_hi ? bounds[w].x : block_hi;
+    block_lo = bounds[w].y > block_lo ? bounds[w].y : block_lo;
+  }
+  block_hi = __builtin_amdgcn_readfirstlane(block_hi);
+  block_lo = __builtin_amdgcn_readfirstlane(block_lo);
+  auto seen_by_all = [&](int s0, int hi, int lo) {
+    return s0 + kSplit - 1 <= hi && s0 >= sl.lo0 && (s0 >= lo || s0 + kSplit - 1 < sinks);
   };
   for (int i = i0; i < i1; ++i) {
     // This wave's part of tile i has landed; after the barrier everyone's has,
     // and every wave is done with tile i - 1, whose buffer tile i + 1 now takes.
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     lds_barrier();
-    if (i + 1 < i1) stage(i + 1);
+    const uint32_t tb = static_cast<uint32_t>(((i - i0) & 1) * kTileBytes);
     const int s0 = tile_of(i);
-    if (active && s0 <= any_hi && (s0 + kSplit > any_lo || s0 < sinks)) {
-      const bool whole = s0 + kSplit - 1 <= all_hi && s0 >= sl.lo0 &&
-                         (s0 >= all_lo || s0 + kSplit - 1 < sinks);
-      const uint32_t tb = static_cast<uint32_t>(((i - i0) & 1) * kTileBytes);
-      tile(s0, tb, whole);
+    if (__builtin_expect(!seen_by_all(s0, block_hi, block_lo), 0)) {
+      // Zero times an infinite or NaN V is NaN: where a tile has any, the rows that
+      // see its slot get it by addition, and the products take it as zero.
+      unsigned char* v = ring + tb + kSplit * D * 2;
+      uint4* own = reinterpret_cast<uint4*>(v + wave * kGroupBytes) + lane;
+      bool odd = false;
+#pragma unroll 1
+      for (int u = 0; u < 4; ++u) {
+        const uint4 x = own[u * 64];
+        finite_pair(x.x, odd);
+        finite_pair(x.y, odd);
+        finite_pair(x.z, odd);
+        finite_pair(x.w, odd);
+      }
+      if (odd) *odd_tile = 1;
+      __syncthreads();
+      if (*odd_tile) {
+        if (active) {
+#pragma unroll
+          for (int n = 0; n < 2; ++n) add_nonfinite(v, kSplit, s0, sight[n], sinks, quad, acc[n]);
+        }
+        __syncthreads();
+        if (tid == 0) *odd_tile = 0;
+#pragma unroll 1
+        for (int u = 0; u < 4; ++u) {
+          const uint4 x = own[u * 64];
+          own[u * 64] = make_uint4(finite_pair(x.x, odd), finite_pair(x.y, odd), finite_pair(x.z, odd),
+                                   finite_pair(x.w, odd));
+        }
+        __syncthreads();
+      }
     }
+    if (i + 1 < i1) stage(i + 1);
+    if (active && s0 <= any_hi && (s0 + kSplit > any_lo || s0 < sinks))
+      tile(s0, tb, seen_by_all(s0, all_hi, all_lo));
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #pragma unroll
@@ -852,6 +902,8 @@ __global__ __launch_bounds__(kBlock, 2) void paged_attention_kernel(PagedArgs a)
   extern __shared__ __align__(16) unsigned char ring[];  // two staged tiles
   __shared__ int rowpos[kManyRows];
   __shared__ float wm[4][16], wl[4][16];
+  __shared__ int2 bounds[4];
+  __shared__ int odd_tile;
   const int prefix = __builtin_amdgcn_readfirstlane(prefix_slots(a));
   Item it{};
   if (!make_plan(a, prefix, it)) return;
@@ -879,7 +931,7 @@ __global__ __launch_bounds__(kBlock, 2) void paged_attention_kernel(PagedArgs a)
   }
   if (it.rows <= 16 && few) attend_few<1>(a, it, sl, table, rowpos, ring, wm, wl);
   else if (few) attend_few<2>(a, it, sl, table, rowpos, ring, wm, wl);
-  else attend_many(a, it, sl, table, rowpos, ring);
+  else attend_many(a, it, sl, table, rowpos, ring, bounds, &odd_tile);
 }
 
 // The rows whose slots were split, one wave each:
