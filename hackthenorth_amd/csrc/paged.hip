@@ -363,20 +363,58 @@ __device__ __forceinline__ Group group_of(const PagedArgs& a, const int32_t* tab
   return g;
 }
 
-// This wave's 16 slots of a tile, K then V, by eight 1 KB LDS-direct loads; rows
-// rotated through the source offsets (K by one 16-byte chunk a slot, V by two),
-// so that the operand reads spread over the banks.
+// A staged row's sixteen 16-byte chunks are rotated by two a slot, chunk c of slot
+// s at (c + 2 s) % 16, through the loads' source offsets, so that the operand reads
+// (one chunk of 16 slots, or four chunks' parts of four) spread over the banks. The
+// offsets of slots 8 further are 2048 bytes on.
+__device__ __forceinline__ void stage_offsets(int lane, uint32_t (&off)[2]) {
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int s = 4 * u + (lane >> 4);
+    off[u] = static_cast<uint32_t>(s * 256 + (((lane & 15) - 2 * s) & 15) * 16);
+  }
+}
+
+// This wave's 16 slots of a tile, K then V, by eight 1 KB LDS-direct loads.
 __device__ __forceinline__ void stage_group(const PagedArgs& a, const Group& g, unsigned char* k_lds,
-                                            unsigned char* v_lds, const uint32_t (&kvoff)[4],
-                                            const uint32_t (&vvoff)[4]) {
+                                            unsigned char* v_lds, const uint32_t (&off)[2]) {
   const __amdgpu_buffer_rsrc_t krs = uniform_rsrc(a.keys + g.offset, g.bytes);
   const __amdgpu_buffer_rsrc_t vrs = uniform_rsrc(a.values + g.offset, g.bytes);
 #pragma unroll
   for (int u = 0; u < 4; ++u)
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(krs, (lds_void_t*)(k_lds + u * 1024), 16, kvoff[u], 0, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(krs, (lds_void_t*)(k_lds + u * 1024), 16, off[u & 1] + (u >> 1) * 2048,
+                                             0, 0, 0);
 #pragma unroll
   for (int u = 0; u < 4; ++u)
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(vrs, (lds_void_t*)(v_lds + u * 1024), 16, vvoff[u], 0, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(vrs, (lds_void_t*)(v_lds + u * 1024), 16, off[u & 1] + (u >> 1) * 2048,
+                                             0, 0, 0);
+}
+
+// Addresses of the operand reads in a tile whose K rows start at LDS byte k and V
+// rows at v (multiples of 256): K chunk 4 ks + quad of slot col, and for the V^T
+// transpose reads, of slot r = 4 quad + col / 4, dims 16 j + 4 (col % 4) .. + 3: 8
+// bytes of chunk 2 j + (col % 4) / 2. Steps ks + 2 and j + 4 are 8 chunks on: bit
+// 7 of the address turned.
+struct ReadAddrs {
+  uint32_t k[2], v[4];
+};
+
+__device__ __forceinline__ ReadAddrs read_addrs(uint32_t k, uint32_t v, int col, int quad) {
+  ReadAddrs r;
+#pragma unroll
+  for (int ks = 0; ks < 2; ++ks)
+    r.k[ks] = k + static_cast<uint32_t>(col * 256 + ((4 * ks + quad + 2 * col) & 15) * 16);
+  const int s = 4 * quad + (col >> 2);
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    r.v[j] = v + static_cast<uint32_t>(s * 256 + ((2 * j + ((col & 3) >> 1) + 2 * s) & 15) * 16 + (col & 1) * 8);
+  return r;
+}
+__device__ __forceinline__ uint32_t k_addr(const ReadAddrs& r, int ks, uint32_t tile) {
+  return (r.k[ks & 1] ^ (ks & 2 ? 128u : 0u)) + tile;
+}
+__device__ __forceinline__ uint32_t v_addr(const ReadAddrs& r, int j, uint32_t tile) {
+  return (r.v[j & 3] ^ (j & 4 ? 128u : 0u)) + tile;
 }
 
 // What a query row sees: slots vlo .. vhi and those below `sinks`.
@@ -457,12 +495,25 @@ __device__ __forceinline__ void settle(f32x4_t (&s)[2][4]) {
 }
 
 // Token and head of row r of an item's row tile.
-__device__ __forceinline__ void row_of(const PagedArgs& a, const Item& it, int tile_rows, int r, int& t,
-                                       int& h) {
+__device__ __forceinline__ void row_of(int group, const Item& it, int tile_rows, int r, int& t, int& h) {
   const int rr = it.tile * tile_rows + r;
-  t = it.t0 + rr / a.G;
-  h = it.kvh * a.G + rr % a.G;
+  t = it.t0 + rr / group;
+  h = it.kvh * group + rr % group;
 }
+
+// The kernel's arguments read anew: what only the end of a block needs would
+// otherwise stay in scalar registers, or spill from them, through its tile loop.
+typedef const __attribute__((address_space(4))) PagedArgs* late_args_t;
+__device__ __forceinline__ late_args_t late_args() {
+  uintptr_t p = (uintptr_t)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return (late_args_t)p;
+}
+
+// The reference that weights are taken against moves only when a row's maximum has
+// outgrown it by 2^kSlack: the sums have room for that, and most tiles then leave
+// the accumulators alone.
+constexpr float kSlack = 8.f;
 
 // Up to 32 query rows (one token of a sequence, or a few): the four waves split
 // the slots, 16 of each tile, and each runs a softmax of its own over them; the
@@ -489,7 +540,7 @@ __device__ __forceinline__ void attend_few(const PagedArgs& a, const Item& it, c
   for (int n = 0; n < NT; ++n) {
     const int r = 16 * n + col;
     int t, h;
-    row_of(a, it, kFewRows, r < it.rows ? r : 0, t, h);  // padding columns repeat row 0
+    row_of(a.G, it, kFewRows, r < it.rows ? r : 0, t, h);  // padding columns repeat row 0
     const bf16_t* qrow = a.q + t * a.q_st + h * a.q_sh + 8 * quad;
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) qf[n][ks] = *reinterpret_cast<const u32x4*>(qrow + 32 * ks);
@@ -498,13 +549,8 @@ __device__ __forceinline__ void attend_few(const PagedArgs& a, const Item& it, c
     all_hi = lo < all_hi ? lo : all_hi;
     all_lo = hi > all_lo ? hi : all_lo;
   }
-  uint32_t kvoff[4], vvoff[4];
-#pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    const int s = 4 * u + (lane >> 4);
-    kvoff[u] = static_cast<uint32_t>(s * 256 + (((lane & 15) - s) & 15) * 16);
-    vvoff[u] = static_cast<uint32_t>(s * 256 + (((lane & 15) - 2 * (s & 7)) & 15) * 16);
-  }
+  uint32_t off[2];
+  stage_offsets(lane, off);
   unsigned char* lds = ring + wave * 2 * kGroupBytes;
   auto slot_of = [&](int i) {
     return (i < sl.sink_tiles ? i : i - sl.sink_tiles + sl.first_tile) * kSplit + wave * 16;
@@ -515,7 +561,7 @@ __device__ __forceinline__ void attend_few(const PagedArgs& a, const Item& it, c
     Group g{0, 0};
     if (i < i1) g = group_of(a, table, it.kvh, slot_of(i), sl.lo0, sl.hi);
     unsigned char* b = lds + ((i - i0) % kRing) * kTileBytes;
-    stage_group(a, g, b, b + kGroupBytes, kvoff, vvoff);
+    stage_group(a, g, b, b + kGroupBytes, off);
   };
   __builtin_amdgcn_sched_barrier(0);
   if (i0 < i1) {
@@ -523,16 +569,7 @@ __device__ __forceinline__ void attend_few(const PagedArgs& a, const Item& it, c
     for (int i = 0; i < kRing; ++i) stage(i0 + i);
   }
   const uint32_t base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void_t*)lds));
-  uint32_t kaddr[4], vaddr[8];
-#pragma unroll
-  for (int ks = 0; ks < 4; ++ks)
-    kaddr[ks] = base + static_cast<uint32_t>(col * 256 + (((4 * ks + quad + col) & 15) * 16));
-  const int vr = 4 * quad + (col >> 2);
-#pragma unroll
-  for (int j = 0; j < 8; ++j)
-    vaddr[j] = base + kGroupBytes +
-               static_cast<uint32_t>(vr * 256 + (((2 * j + ((col & 3) >> 1) + 2 * (vr & 7)) & 15) * 16) +
-                                     (col & 1) * 8);
+  const ReadAddrs from = read_addrs(base, base + kGroupBytes, col, quad);
   f32x4_t acc[NT][8];
   float m[NT], l[NT];
 #pragma unroll
@@ -552,12 +589,12 @@ __device__ __forceinline__ void attend_few(const PagedArgs& a, const Item& it, c
         "ds_read_b128 %2, %7\n\t"
         "ds_read_b128 %3, %8"
         : "=&v"(k[0]), "=&v"(k[1]), "=&v"(k[2]), "=&v"(k[3])
-        : "n"(8 * (kRing - 1)), "v"(kaddr[0] + ro), "v"(kaddr[1] + ro), "v"(kaddr[2] + ro),
-          "v"(kaddr[3] + ro)
+        : "n"(8 * (kRing - 1)), "v"(k_addr(from, 0, ro)), "v"(k_addr(from, 1, ro)), "v"(k_addr(from, 2, ro)),
+          "v"(k_addr(from, 3, ro))
         : "memory");
     uint32_t va[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) va[j] = vaddr[j] + ro;
+    for (int j = 0; j < 8; ++j) va[j] = v_addr(from, j, ro);
     u32x2_t v[8];
     issue_vt_tr<0>(va, v);
     asm volatile("s_waitcnt lgkmcnt(0)"
@@ -593,15 +630,16 @@ __device__ __forceinline__ void attend_few(const PagedArgs& a, const Item& it, c
         }
       }
       const float tmax = quad_max(fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])));
-      const float m_new = fmaxf(m[n], tmax);
-      const float ms = m_new == -INFINITY ? 0.f : m_new;  // nothing visible yet: weights of 0
-      if (!__all(m_new == m[n])) {
-        const float alpha = __builtin_amdgcn_exp2f(m[n] - ms);
+      const bool moves = tmax > m[n] + kSlack;  // see kSlack
+      if (__any(moves)) {
+        const float m_new = moves ? tmax : m[n];
+        const float alpha = __builtin_amdgcn_exp2f(m[n] - (m_new == -INFINITY ? 0.f : m_new));
         l[n] *= alpha;
 #pragma unroll
         for (int j = 0; j < 8; ++j) acc[n][j] *= alpha;
+        m[n] = m_new;
       }
-      m[n] = m_new;
+      const float ms = m[n] == -INFINITY ? 0.f : m[n];  // nothing visible yet: weights of 0
       float p[4];
 #pragma unroll
       for (int r = 0; r < 4; ++r) p[r] = __builtin_amdgcn_exp2f(sc[r] - ms);
@@ -617,6 +655,7 @@ __device__ __forceinline__ void attend_few(const PagedArgs& a, const Item& it, c
   }
   // The waves' states, in LDS rows of 132 floats (the 16 rows in other banks).
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  const late_args_t la = late_args();
   float* wacc = reinterpret_cast<float*>(ring);
   constexpr int kRowFloats = D + 4;
 #pragma unroll
@@ -646,13 +685,13 @@ __device__ __forceinline__ void attend_few(const PagedArgs& a, const Item& it, c
       }
       if (it.part >= 0) {
         const long row = it.part + 16 * n + c;
-        *reinterpret_cast<float2*>(a.part + row * D + 2 * lane) = make_float2(x, y);
-        if (lane == 0) a.ml[row] = make_float2(M, L);
+        *reinterpret_cast<float2*>(la->part + row * D + 2 * lane) = make_float2(x, y);
+        if (lane == 0) la->ml[row] = make_float2(M, L);
       } else {
         int tr, hr;
-        row_of(a, it, kFewRows, 16 * n + c, tr, hr);
+        row_of(la->G, it, kFewRows, 16 * n + c, tr, hr);
         const float inv = M == -INFINITY ? 0.f : 1.0f / L;
-        *reinterpret_cast<uint32_t*>(a.out + tr * a.o_st + hr * a.o_sh + 2 * lane) = pack_bf2(x * inv, y * inv);
+        *reinterpret_cast<uint32_t*>(la->out + tr * la->o_st + hr * la->o_sh + 2 * lane) = pack_bf2(x * inv, y * inv);
       }
     }
   }
@@ -680,7 +719,7 @@ __device__ __forceinline__ void attend_many(const PagedArgs& a, const Item& it, 
   for (int n = 0; n < 2; ++n) {
     const int r = 32 * wave + 16 * n + col;
     int t, h;
-    row_of(a, it, kManyRows, r < it.rows ? r : it.rows - 1, t, h);
+    row_of(a.G, it, kManyRows, r < it.rows ? r : it.rows - 1, t, h);
     const bf16_t* qrow = a.q + t * a.q_st + h * a.q_sh + 8 * quad;
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) qf[n][ks] = *reinterpret_cast<const u32x4*>(qrow + 32 * ks);
@@ -693,37 +732,24 @@ __device__ __forceinline__ void attend_many(const PagedArgs& a, const Item& it, 
     any_hi = top > any_hi ? top : any_hi;
     any_lo = low < any_lo ? low : any_lo;
   }
-  uint32_t kvoff[4], vvoff[4];
-#pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    const int s = 4 * u + (lane >> 4);
-    kvoff[u] = static_cast<uint32_t>(s * 256 + (((lane & 15) - s) & 15) * 16);
-    vvoff[u] = static_cast<uint32_t>(s * 256 + (((lane & 15) - 2 * (s & 7)) & 15) * 16);
-  }
+  uint32_t off[2];
+  stage_offsets(lane, off);
   auto tile_of = [&](int i) {
     return (i < sl.sink_tiles ? i : i - sl.sink_tiles + sl.first_tile) * kSplit;
   };
   auto stage = [&](int i) {
     const Group g = group_of(a, table, it.kvh, tile_of(i) + wave * 16, sl.lo0, sl.hi);
     unsigned char* b = ring + ((i - i0) & 1) * kTileBytes + wave * kGroupBytes;
-    stage_group(a, g, b, b + kSplit * D * 2, kvoff, vvoff);
+    stage_group(a, g, b, b + kSplit * D * 2, off);
   };
   __builtin_amdgcn_sched_barrier(0);
   if (i0 < i1) stage(i0);
   const uint32_t ring_base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void_t*)ring));
-  uint32_t kaddr[4], vaddr[8];
-#pragma unroll
-  for (int ks = 0; ks < 4; ++ks)
-    kaddr[ks] = ring_base + static_cast<uint32_t>(col * 256 + (((4 * ks + quad + col) & 15) * 16));
-  const int vr = 4 * quad + (col >> 2);
-#pragma unroll
-  for (int j = 0; j < 8; ++j)
-    vaddr[j] = ring_base + kSplit * D * 2 +
-               static_cast<uint32_t>(vr * 256 + (((2 * j + ((col & 3) >> 1) + 2 * (vr & 7)) & 15) * 16) +
-                                     (col & 1) * 8);
+  const ReadAddrs from = read_addrs(ring_base, ring_base + kSplit * D * 2, col, quad);
   const u32x4 ones = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
   f32x4_t acc[2][8], sum[2];
-  float m[2] = {-INFINITY, -INFINITY};  // of the unscaled scores
+  float m[2] = {-INFINITY, -INFINITY}, base[2] = {0.f, 0.f};  // of the unscaled scores, and scaled
+  const float slack = kSlack / a.scale2;
 #pragma unroll
   for (int n = 0; n < 2; ++n) {
     sum[n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -737,10 +763,10 @@ __device__ __forceinline__ void attend_many(const PagedArgs& a, const Item& it, 
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) st[n][mt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     u32x4 kf[4][4];
-    issue_k_pf<0>(kaddr[0] + tb, kf[0]);
-    issue_k_pf<0>(kaddr[1] + tb, kf[1]);
-    issue_k_pf<0>(kaddr[2] + tb, kf[2]);
-    issue_k_pf<0>(kaddr[3] + tb, kf[3]);
+    issue_k_pf<0>(k_addr(from, 0, tb), kf[0]);
+    issue_k_pf<0>(k_addr(from, 1, tb), kf[1]);
+    issue_k_pf<0>(k_addr(from, 2, tb), kf[2]);
+    issue_k_pf<0>(k_addr(from, 3, tb), kf[3]);
     wait_k16(kf);
 #pragma unroll
     for (int n = 0; n < 2; ++n)
@@ -751,7 +777,7 @@ __device__ __forceinline__ void attend_many(const PagedArgs& a, const Item& it, 
     // The V^T operands of half the tile in flight during the softmax.
     uint32_t va[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) va[j] = vaddr[j] + tb;
+    for (int j = 0; j < 8; ++j) va[j] = v_addr(from, j, tb);
     u32x2_t vw[2][8];
     issue_vt_tr<0>(va, vw[0]);
     issue_vt_tr<4096>(va, vw[1]);
@@ -760,6 +786,7 @@ __device__ __forceinline__ void attend_many(const PagedArgs& a, const Item& it, 
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
       if (!whole) {
+        asm volatile("");  // a branch, not 16 selects on every tile
 #pragma unroll
         for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
@@ -773,21 +800,23 @@ __device__ __forceinline__ void attend_many(const PagedArgs& a, const Item& it, 
       for (int i = 3; i < 15; i += 2)
         tmax = max3(tmax, st[n][i / 4][i % 4], st[n][(i + 1) / 4][(i + 1) % 4]);
       tmax = quad_max(fmaxf(tmax, st[n][3][3]));
-      const float m_new = fmaxf(m[n], tmax);
-      const float ms = m_new == -INFINITY ? 0.f : m_new * a.scale2;
-      if (!__all(m_new == m[n])) {
+      const bool moves = tmax > m[n] + slack;  // see kSlack
+      if (__any(moves)) {
+        const float m_new = moves ? tmax : m[n];  // of that row alone: no row's sums depend on another's scores
+        const float ms = m_new == -INFINITY ? 0.f : m_new * a.scale2;  // nothing visible yet: weights of 0
         // Not 0, so that an infinity that was added stays one.
         const float alpha = fmaxf(__builtin_amdgcn_exp2f(fmaf(m[n], a.scale2, -ms)), 1.2e-38f);
         sum[n] *= alpha;
 #pragma unroll
         for (int j = 0; j < 8; ++j) acc[n][j] *= alpha;
+        m[n] = m_new;
+        base[n] = ms;
       }
-      m[n] = m_new;
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) {
         float p[4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) p[r] = __builtin_amdgcn_exp2f(fmaf(st[n][mt][r], a.scale2, -ms));
+        for (int r = 0; r < 4; ++r) p[r] = __builtin_amdgcn_exp2f(fmaf(st[n][mt][r], a.scale2, -base[n]));
         pb[n][mt] = make_uint2(pack_bf2(p[0], p[1]), pack_bf2(p[2], p[3]));
       }
     }
@@ -874,6 +903,7 @@ __device__ __forceinline__ void attend_many(const PagedArgs& a, const Item& it, 
       tile(s0, tb, seen_by_all(s0, all_hi, all_lo));
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  const late_args_t la = late_args();
 #pragma unroll
   for (int n = 0; n < 2; ++n) {
     const int r = 32 * wave + 16 * n + col;
@@ -883,13 +913,13 @@ __device__ __forceinline__ void attend_many(const PagedArgs& a, const Item& it, 
       const long row = it.part + r;
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        *reinterpret_cast<f32x4_t*>(a.part + row * D + 16 * j + 4 * quad) = acc[n][j];
-      if (quad == 0) a.ml[row] = make_float2(none ? -INFINITY : m[n] * a.scale2, sum[n][0]);
+        *reinterpret_cast<f32x4_t*>(la->part + row * D + 16 * j + 4 * quad) = acc[n][j];
+      if (quad == 0) la->ml[row] = make_float2(none ? -INFINITY : m[n] * la->scale2, sum[n][0]);
     } else {
       int t, h;
-      row_of(a, it, kManyRows, r, t, h);
+      row_of(la->G, it, kManyRows, r, t, h);
       const float inv = none ? 0.f : 1.0f / sum[n][0];
-      bf16_t* dst = a.out + t * a.o_st + h * a.o_sh + 4 * quad;
+      bf16_t* dst = la->out + t * la->o_st + h * la->o_sh + 4 * quad;
 #pragma unroll
       for (int j = 0; j < 8; ++j)
         *reinterpret_cast<uint2*>(dst + 16 * j) = make_uint2(pack_bf2(acc[n][j][0] * inv, acc[n][j][1] * inv),
@@ -899,7 +929,7 @@ __device__ __forceinline__ void attend_many(const PagedArgs& a, const Item& it, 
 }
 
 __global__ __launch_bounds__(kBlock, 2) void paged_attention_kernel(PagedArgs a) {
-  extern __shared__ __align__(16) unsigned char ring[];  // two staged tiles
+  extern __shared__ __align__(256) unsigned char ring[];  // two staged tiles
   __shared__ int rowpos[kManyRows];
   __shared__ float wm[4][16], wl[4][16];
   __shared__ int2 bounds[4];
