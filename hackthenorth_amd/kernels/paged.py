@@ -25,6 +25,7 @@ import torch
 from .. import _lib
 
 _BF16, _I32, _I64 = torch.bfloat16, torch.int32, torch.int64
+_PACKED = torch.contiguous_format
 _PAGES = tuple(16 << i for i in range(7))
 
 
@@ -130,7 +131,7 @@ def norm_rope_paged(q, k, v, q_norm, k_norm, cos, sin, key_pages, value_pages, p
     batch, row_st, row_pages = _check_batch(page_table, query_starts, lengths)
     index = _place(q, k, v, q_gain, k_gain, cos, sin, key_pages, value_pages, page_table,
                    query_starts, lengths)
-    out = torch.empty(shape, dtype=_BF16, device=q.device)
+    out = torch.empty_like(q, memory_format=_PACKED)
     _launch("htn_norm_rope_paged", index, q.data_ptr(), q_st[0], k.data_ptr(), k_st[0],
             v.data_ptr(), v_st[0], _lib.ptr(q_gain), _lib.ptr(k_gain), q_eps, k_eps,
             cos.data_ptr(), sin.data_ptr(), table_st[0], table_shape[0], kind is torch.float32,
@@ -152,14 +153,13 @@ def _attend(name, q, key_pages, value_pages, prefix, page_table, query_starts, l
     if out is not None and (out.shape != shape or out.dtype is not _BF16 or out.stride(2) != 1):
         raise ValueError("out must be a bf16 view shaped like q with unit dim stride")
     index = _place(q, key_pages, value_pages, page_table, query_starts, lengths, out, *prefix)
-    device = q.device
     if out is None:
-        out = torch.empty(shape, dtype=_BF16, device=device)
+        out = torch.empty_like(q, memory_format=_PACKED)
         out_t, out_h = heads * _lib.HEAD_DIM, _lib.HEAD_DIM
     else:
         out_t, out_h, _ = out.stride()
     nbytes = _scratch_bytes(tokens, batch, heads, kv_heads, bool(prefix))
-    scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
     before = (prefix[0].data_ptr(), prefix[0].numel(), prefix[1].data_ptr()) if prefix else ()
     _launch(name, index, q.data_ptr(), strides[0], strides[1], key_pages.data_ptr(),
             value_pages.data_ptr(), pages, page, *before, page_table.data_ptr(), row_st, row_pages,

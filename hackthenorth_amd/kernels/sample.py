@@ -58,7 +58,9 @@ def sample_token(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0
     p, p_all = _setting(top_p, "top_p", rows, torch.float32, 0.0)
     m, m_all = _setting(min_p, "min_p", rows, torch.float32, 0.0)
     if out is None:
-        out = torch.empty(shape[:-1], dtype=torch.int64, device=logits.device)
+        out = torch.empty(rows, dtype=torch.int64, device=logits.device)
+        if len(shape) != 2:
+            out = out.view(shape[:-1])
     elif out.dtype != torch.int64 or out.shape != shape[:-1] or not out.is_contiguous():
         raise ValueError("out must be contiguous int64 with one entry per row")
     index = _place(flat, uniform, heat, k, p, m, out)
