@@ -23,6 +23,13 @@
 //      finer bins and by rank. More than 2048 tokens (a flat row, or many equal
 //      logits) are read again from the row for the one border, narrowed by eight
 //      bits of (logit, id) at a time.
+//
+// One row of 151936 bf16 logits takes 27 us: five launches of 3, 5, 6, 4.5 and
+// 10 us, each a chain of loads, scans and barriers. 64 such rows in fp32 (39 MB)
+// take 56: 6.5, 15, 9, 11 and 15 us, the second bound by the 64-bit additions to LDS
+// bins. Steps 2 + 3 and 4 + 5 in one launch each, by the row's last block, save one
+// row 2.5 us and cost 64 rows 12; steps 3 + 4, each block planning for itself, 1.6
+// and 2 to 20.
 #include "common.h"
 
 namespace htn {
@@ -700,7 +707,8 @@ struct Layout {
 
 Layout layout_of(long rows, long vocab) {
   Layout l;
-  // Two blocks a CU where the chunks stay at 2048 tokens or more.
+  // Two blocks a CU where the chunks stay at 2048 tokens or more, 16 a row at most
+  // (8: one row 28.8 us instead of 27.2).
   long c = 512 / rows;
   const long most = (vocab + 2047) / 2048, fewest = (vocab + kChunk - 1) / kChunk;
   c = c < most ? c : most;
