@@ -513,6 +513,10 @@ __device__ __forceinline__ late_args_t late_args() {
   return (late_args_t)p;
 }
 
+// What earlier sums weigh against later ones, 2^x. Not 0, so that an infinity or a NaN
+// in them stays one.
+__device__ __forceinline__ float share(float x) { return fmaxf(__builtin_amdgcn_exp2f(x), 1.2e-38f); }
+
 // The reference that weights are taken against moves only when a row's maximum has
 // outgrown it by 2^kSlack: the sums have room for that, and most tiles then leave
 // the accumulators alone (5000-token prompt 250 -> 240 us).
@@ -643,7 +647,7 @@ __device__ __forceinline__ void attend_few(const PagedArgs& a, const Item& it, c
       const bool moves = tmax > m[n] + kSlack;  // see kSlack
       if (__any(moves)) {
         const float m_new = moves ? tmax : m[n];
-        const float alpha = __builtin_amdgcn_exp2f(m[n] - (m_new == -INFINITY ? 0.f : m_new));
+        const float alpha = share(m[n] - (m_new == -INFINITY ? 0.f : m_new));
         l[n] *= alpha;
 #pragma unroll
         for (int j = 0; j < 8; ++j) acc[n][j] *= alpha;
@@ -686,7 +690,7 @@ __device__ __forceinline__ void attend_few(const PagedArgs& a, const Item& it, c
       if (M != -INFINITY) {
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-          const float f = __builtin_amdgcn_exp2f(wm[w][c] - M);
+          const float f = share(wm[w][c] - M);
           const float2 o = *reinterpret_cast<const float2*>(wacc + (w * 16 + c) * kRowFloats + 2 * lane);
           L = fmaf(f, wl[w][c], L);
           x = fmaf(f, o.x, x);
@@ -822,8 +826,7 @@ __device__ __forceinline__ void attend_many(const PagedArgs& a, const Item& it, 
       if (__any(moves)) {
         const float m_new = moves ? tmax : m[n];  // of that row alone: no row's sums depend on another's scores
         const float ms = m_new == -INFINITY ? 0.f : m_new * a.scale2;  // nothing visible yet: weights of 0
-        // Not 0, so that an infinity that was added stays one.
-        const float alpha = fmaxf(__builtin_amdgcn_exp2f(fmaf(m[n], a.scale2, -ms)), 1.2e-38f);
+        const float alpha = share(fmaf(m[n], a.scale2, -ms));
         sum[n] *= alpha;
 #pragma unroll
         for (int j = 0; j < 8; ++j) acc[n][j] *= alpha;
@@ -1015,8 +1018,8 @@ __global__ __launch_bounds__(kBlock) void paged_merge_kernel(PagedArgs a) {
         const float2 ml = lane < n ? a.ml[row + (c0 + lane) * step] : make_float2(-INFINITY, 0.f);
         const float mb = fmaxf(M, wave_max(ml.x));
         if (mb == -INFINITY) continue;
-        const float f0 = __builtin_amdgcn_exp2f(M - mb);
-        const float f = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - mb);
+        const float f0 = share(M - mb);
+        const float f = ml.x == -INFINITY ? 0.f : share(ml.x - mb);
         M = mb;
         L = fmaf(L, f0, wave_sum(f * ml.y));
         o *= f0;

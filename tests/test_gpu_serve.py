@@ -170,6 +170,37 @@ def test_captured_decode_loop_equals_the_eager_one(shared):
     assert torch.equal(eager.server.values, replayed.server.values)
 
 
+@pytest.mark.parametrize("new,length,shared", [(1, 2000, 0), (3, 300, 0), (40, 1500, 0), (200, 2600, 0),
+                                               (1, 1400, 512), (50, 1400, 1040)])
+def test_infinite_value_of_a_slot_without_weight(new, length, shared):
+    """The first 1024 slots' scores lie some 900 below the others', their weights below
+    what 32 bits hold; an infinite V there still reaches the rows, and no other dim."""
+    g = torch.Generator().manual_seed(21)
+    pages, low = -(-length // PAGE), min(1024, length // 2)
+    keys, values = (torch.randn(pages, KV, PAGE, D, generator=g).to(torch.bfloat16) for _ in range(2))
+    keys.view(pages, KV, PAGE, D)[:low // PAGE] = -40.0
+    q = torch.full((new, HEADS, D), 2.0, dtype=torch.bfloat16).cuda()
+    table = torch.arange(pages, dtype=torch.int32)[None].cuda()
+    starts, lengths = torch.tensor([0, new]).cuda(), torch.tensor([length]).cuda()
+    keys, values = keys.cuda(), values.cuda()
+
+    def run():
+        if shared:
+            return shared_prefix_attention(q, keys, values, table[0, :shared // PAGE].contiguous(),
+                                           torch.tensor([shared]).cuda(), table, starts, lengths)
+        return paged_attention(q, keys, values, table, starts, lengths)
+    clean = run()
+    for slot in (0, 37, low - PAGE - 1):
+        kept = values[slot // PAGE, 0, slot % PAGE, 5].clone()
+        values[slot // PAGE, 0, slot % PAGE, 5] = float("inf")
+        got = run()
+        values[slot // PAGE, 0, slot % PAGE, 5] = kept
+        assert not bool(got[:, :HEADS // KV, 5].isfinite().any())
+        other = [d for d in range(D) if d != 5]
+        assert torch.equal(got[..., other], clean[..., other])
+        assert torch.equal(got[:, HEADS // KV:], clean[:, HEADS // KV:])
+
+
 def test_two_streams_at_once():
     """Two servers' steps, each on a stream of its own, as one after the other."""
     model = Model()
