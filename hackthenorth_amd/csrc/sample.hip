@@ -468,8 +468,14 @@ __global__ __launch_bounds__(kThreads) void sample_collect(SampleArgs a) {
   if (tid < kBorders) a.listed[at * kBorders + tid] = taken[tid];
 }
 
+struct Found {
+  uint64_t weight;  // of the tokens up to and with the one at the border
+  uint32_t id;      // that token
+};
+
 struct Shared {
   Ranks ranks;
+  Found found;
   uint64_t keys[kBorders][kListed], near[kThreads];
   uint32_t fine_count[kThreads];
   unsigned long long fine_weight[kThreads];
@@ -514,7 +520,6 @@ __device__ __forceinline__ void sort_keys(uint64_t* keys, int n) {
 // row, `weight` before the bin and `sum` before them in it.
 struct Place {
   int bin;
-  double unit;
   uint32_t here, count;
   uint64_t weight, sum;
 };
@@ -527,8 +532,9 @@ __device__ __forceinline__ void narrow(Ranks& s, Place& p, const Border& b, uint
   scan(s, c1, s1);
   const uint64_t s0 = p.sum + s1 - sum;
   s1 += p.sum;
-  find_border(s, b, p.count + c1 - count, p.weight + outside(s0, p.unit), p.count + c1,
-              p.weight + outside(s1, p.unit), p.count + p.here);
+  const double unit = unit_of(p.bin);
+  find_border(s, b, p.count + c1 - count, p.weight + outside(s0, unit), p.count + c1,
+              p.weight + outside(s1, unit), p.count + p.here);
   if (threadIdx.x == s.at) s.weight_before = s0;
   __syncthreads();
   p.count = s.count_before;
@@ -536,10 +542,6 @@ __device__ __forceinline__ void narrow(Ranks& s, Place& p, const Border& b, uint
   p.sum = s.weight_before;
 }
 
-struct Found {
-  uint64_t weight;  // of the tokens up to and with the one at the border
-  uint32_t id;      // that token
-};
 
 __device__ __forceinline__ uint64_t key_weight(const Row& w, uint64_t key, int bin) {
   return weight_in_bin(past_edge(w, key_logit(key), bin));
@@ -551,6 +553,31 @@ __device__ __forceinline__ Found among(Shared& s, const Row& w, uint64_t* keys, 
   sort_keys(keys, n);
   narrow(s.ranks, p, b, tid < n ? 1u : 0u, tid < n ? key_weight(w, keys[tid], p.bin) : 0);
   return Found{s.ranks.weight_with, 0xffffffffu - static_cast<uint32_t>(keys[s.ranks.at] & 0xffffffffu)};
+}
+
+// The same among p.here <= 64 keys, by the first wave alone: the others wait at one
+// barrier instead of taking their turns at scans and at eight.
+__device__ __forceinline__ Found among_few(Shared& s, const Row& w, uint64_t* keys, const Place& p, const Border& b) {
+  const int lane = threadIdx.x & 63, n = p.here;
+  __syncthreads();
+  if (threadIdx.x < kWave) {
+    uint64_t key = lane < n ? keys[lane] : 0;
+    int rank = 0;
+#pragma unroll 8
+    for (int i = 0; i < n; ++i) rank += keys[i] > key;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (lane < n) keys[rank] = key;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    key = lane < n ? keys[lane] : 0;
+    const uint64_t own = lane < n ? key_weight(w, key, p.bin) : 0, s1 = p.sum + wave_scan(own);
+    const double unit = unit_of(p.bin);
+    const uint64_t w0 = p.weight + outside(s1 - own, unit), w1 = p.weight + outside(s1, unit);
+    const uint32_t c0 = p.count + lane;
+    if (lane < n && !reached(b, c0, w0) && (reached(b, c0 + 1, w1) || lane == n - 1))
+      s.found = Found{w1, 0xffffffffu - static_cast<uint32_t>(key & 0xffffffffu)};
+  }
+  __syncthreads();
+  return s.found;
 }
 
 // Narrows a place to 1024 tokens at most, its tokens read from the row again, eight
@@ -653,9 +680,22 @@ __global__ __launch_bounds__(kThreads) void sample_pick(SampleArgs a) {
     const Border b = i == 0 ? Border{kCount, static_cast<uint64_t>(set.top_k), 0.0}
                             : (i == 1 ? border_p(set, kept) : border_u(set, least(kept, plan.floor_p)));
     find_border(s.ranks, b, c0, w0, c1, w1, all_c);
-    Place p{s.ranks.at, unit_of(s.ranks.at), s.ranks.here, s.ranks.count_before, s.ranks.weight_before, 0};
+    Place p{s.ranks.at, s.ranks.here, s.ranks.count_before, s.ranks.weight_before, 0};
     const uint32_t listed = s.ends[i][kMaxChunks - 1];
     bool whole = listed > 0;
+    if (whole && p.here <= kWave) {
+      if (tid == 0) s.taken = 0;
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) {
+        const uint32_t at = tid + j * kThreads;
+        if (at < listed && bin_of(w, key_logit(s.keys[i][at])) == p.bin)
+          s.near[atomicAdd(&s.taken, 1u)] = s.keys[i][at];
+      }
+      f = among_few(s, w, s.near, p, b);
+      kept = i < 2 ? least(kept, f.weight) : kept;
+      continue;
+    }
     int only = -1;
     int fine[kEach];
     if (whole) {
@@ -673,28 +713,25 @@ __global__ __launch_bounds__(kThreads) void sample_pick(SampleArgs a) {
         if (bin_of(w, x) != p.bin) continue;
         const double y = past_edge(w, x, p.bin), g = y * kThreads;
         fine[j] = g > 0.0 ? (g < kThreads - 1 ? static_cast<int>(g) : kThreads - 1) : 0;
-        if (p.here <= 64) continue;
         atomicAdd(&s.fine_count[fine[j]], 1u);
         atomicAdd(&s.fine_weight[fine[j]], static_cast<unsigned long long>(weight_in_bin(y)));
       }
       __syncthreads();
-      if (p.here > 64) {
-        Place q = p;
-        narrow(s.ranks, q, b, s.fine_count[tid], s.fine_weight[tid]);
-        only = s.ranks.at;
-        whole = q.here <= kThreads;
-        if (whole) p = q;
-      }
+      Place q = p;
+      narrow(s.ranks, q, b, s.fine_count[tid], s.fine_weight[tid]);
+      only = s.ranks.at;
+      whole = q.here <= kThreads;
+      if (whole) p = q;
     }
     if (whole) {
 #pragma unroll
       for (int j = 0; j < kEach; ++j)
-        if (fine[j] >= 0 && (only < 0 || fine[j] == only))
+        if (fine[j] == only)
           s.near[atomicAdd(&s.taken, 1u)] = s.keys[i][tid + j * kThreads];
     } else {
       reread<L>(a, s, w, r, p, b);
     }
-    f = among(s, w, s.near, p, b);
+    f = p.here <= kWave ? among_few(s, w, s.near, p, b) : among(s, w, s.near, p, b);
     kept = i < 2 ? least(kept, f.weight) : kept;
   }
   if (tid == 0) a.out[r] = f.id;
