@@ -20,9 +20,10 @@
 //      borders, only within its bin's);
 //   4. every chunk: its tokens in these bins as lists;
 //   5. one block a row: each border in turn, its bin and then its tokens, by 1024
-//      finer bins and by rank. More than 2048 tokens (a flat row, or many equal
-//      logits) are read again from the row for the one border, narrowed by eight
-//      bits of (logit, id) at a time.
+//      finer bins and by rank. Lists of more than 2048 tokens stay in memory; where
+//      a chunk's own passes that, or a finer bin holds more than 1024 tokens (a flat
+//      row, or many equal logits), the bin's tokens are read again from the row,
+//      narrowed by eight bits of (logit, id) at a time.
 //
 // One row of 151936 bf16 logits takes 27 us: five launches of 3, 5, 6, 4.5 and
 // 10 us, each a chain of loads, scans and barriers. 64 such rows in fp32 (39 MB)
@@ -39,7 +40,7 @@ namespace {
 constexpr int kThreads = 1024;
 constexpr int kWaves = kThreads / kWave;
 constexpr int kBins = 1024;        // one a thread
-constexpr int kListed = 2048;      // tokens listed for a border
+constexpr int kListed = 2048;      // tokens listed for a border, of a chunk
 constexpr int kBorders = 3;        // top-k's, top-p's and the draw's
 constexpr int kMaxChunks = 16;
 constexpr long kChunk = 32760;     // tokens of a chunk at most
@@ -441,7 +442,7 @@ __global__ __launch_bounds__(kThreads) void sample_collect(SampleArgs a) {
 #pragma unroll
   for (int i = 0; i < kBorders; ++i) {
     const Range g = plan.range[i];
-    const bool on = g.hi >= g.lo && g.tokens <= kListed;
+    const bool on = g.hi >= g.lo && g.tokens <= static_cast<uint32_t>(a.chunks) * kListed;
     lo[i] = on ? g.lo : 2 * kBins;  // no bin is in it
     span[i] = on ? g.hi - g.lo : 0;
     any_lo = on && g.lo < any_lo ? g.lo : any_lo;
@@ -461,8 +462,10 @@ __global__ __launch_bounds__(kThreads) void sample_collect(SampleArgs a) {
                        if (bin < any_lo || bin > any_hi) return;
 #pragma unroll
                        for (int i = 0; i < kBorders; ++i)
-                         if (static_cast<uint32_t>(bin - lo[i]) <= span[i])
-                           lists[i * kListed + atomicAdd(&taken[i], 1u)] = order_key(x, id);
+                         if (static_cast<uint32_t>(bin - lo[i]) <= span[i]) {
+                           const uint32_t n = atomicAdd(&taken[i], 1u);
+                           if (n < kListed) lists[i * kListed + n] = order_key(x, id);
+                         }
                      });
   __syncthreads();
   if (tid < kBorders) a.listed[at * kBorders + tid] = taken[tid];
@@ -637,6 +640,7 @@ __global__ __launch_bounds__(kThreads) void sample_pick(SampleArgs a) {
   if (tid < kBorders * kWave) {
     const int i = tid >> 6;
     uint32_t n = lane < a.chunks ? a.listed[(row_at + lane) * kBorders + i] : 0;
+    if (__any(n > kListed)) n = 0;  // a list that did not hold them all is none
 #pragma unroll
     for (int m = 1; m < kMaxChunks; m <<= 1) {
       const uint32_t o = __shfl_up(n, m, kWave);
@@ -651,26 +655,29 @@ __global__ __launch_bounds__(kThreads) void sample_pick(SampleArgs a) {
   }
   const Settings set = settings_of(a, w, r);
   __syncthreads();
-  // All borders' lists at once, the chunks' one after the other.
+  // Key `at` of border i's lists, the chunks' one after the other.
+  auto key_at = [&](int i, uint32_t at) {
+    int c = 0;
+#pragma unroll
+    for (int m = kMaxChunks / 2; m >= 1; m >>= 1)
+      if (s.ends[i][c + m - 1] <= at) c += m;
+    const uint32_t before = c ? s.ends[i][c - 1] : 0;
+    return a.lists[((row_at + c) * kBorders + i) * kListed + at - before];
+  };
+  // All borders' lists that fit the block's memory at once.
   constexpr int kEach = kListed / kThreads;
   uint64_t key[kBorders][kEach];
-#pragma unroll
-  for (int i = 0; i < kBorders; ++i)
-#pragma unroll
-    for (int j = 0; j < kEach; ++j) {
-      const uint32_t at = tid + j * kThreads;
-      int c = 0;  // the chunk whose list the place is in
-#pragma unroll
-      for (int m = kMaxChunks / 2; m >= 1; m >>= 1)
-        if (s.ends[i][c + m - 1] <= at) c += m;
-      const uint32_t before = c ? s.ends[i][c - 1] : 0;
-      if (at < s.ends[i][kMaxChunks - 1]) key[i][j] = a.lists[((row_at + c) * kBorders + i) * kListed + at - before];
-    }
+  auto kept_here = [&](int i) { return s.ends[i][kMaxChunks - 1] <= kListed ? s.ends[i][kMaxChunks - 1] : 0; };
 #pragma unroll
   for (int i = 0; i < kBorders; ++i)
 #pragma unroll
     for (int j = 0; j < kEach; ++j)
-      if (tid + j * kThreads < s.ends[i][kMaxChunks - 1]) s.keys[i][tid + j * kThreads] = key[i][j];
+      if (tid + j * kThreads < kept_here(i)) key[i][j] = key_at(i, tid + j * kThreads);
+#pragma unroll
+  for (int i = 0; i < kBorders; ++i)
+#pragma unroll
+    for (int j = 0; j < kEach; ++j)
+      if (tid + j * kThreads < kept_here(i)) s.keys[i][tid + j * kThreads] = key[i][j];
   uint64_t kept = plan.all;
   Found f{};
 #pragma unroll 1
@@ -682,40 +689,43 @@ __global__ __launch_bounds__(kThreads) void sample_pick(SampleArgs a) {
     find_border(s.ranks, b, c0, w0, c1, w1, all_c);
     Place p{s.ranks.at, s.ranks.here, s.ranks.count_before, s.ranks.weight_before, 0};
     const uint32_t listed = s.ends[i][kMaxChunks - 1];
-    bool whole = listed > 0;
-    if (whole && p.here <= kWave) {
-      if (tid == 0) s.taken = 0;
-      __syncthreads();
+    // g(key, logit) for the listed tokens of the border's bin.
+    auto each_listed = [&](auto&& g) {
+      auto one = [&](uint64_t k) {
+        const float x = key_logit(k);
+        if (bin_of(w, x) == p.bin) g(k, x);
+      };
+      if (listed <= kListed) {
 #pragma unroll
-      for (int j = 0; j < kEach; ++j) {
-        const uint32_t at = tid + j * kThreads;
-        if (at < listed && bin_of(w, key_logit(s.keys[i][at])) == p.bin)
-          s.near[atomicAdd(&s.taken, 1u)] = s.keys[i][at];
+        for (int j = 0; j < kEach; ++j)
+          if (tid + j * kThreads < listed) one(s.keys[i][tid + j * kThreads]);
+        return;
       }
-      f = among_few(s, w, s.near, p, b);
-      kept = i < 2 ? least(kept, f.weight) : kept;
-      continue;
-    }
+      for (uint32_t at = tid; at < listed; at += 4 * kThreads) {
+        uint64_t k[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) k[u] = key_at(i, at + u * kThreads < listed ? at + u * kThreads : at);
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (at + u * kThreads < listed) one(k[u]);
+      }
+    };
+    // The token's place among 1024 finer bins of the bin.
+    auto fine_of = [&](float x) {
+      const double g = past_edge(w, x, p.bin) * kThreads;
+      return g > 0.0 ? (g < kThreads - 1 ? static_cast<int>(g) : kThreads - 1) : 0;
+    };
+    bool whole = listed > 0;
     int only = -1;
-    int fine[kEach];
-    if (whole) {
-      // The bin's own tokens, in 1024 finer bins where they are many.
+    if (whole && p.here > kWave) {
       s.fine_count[tid] = 0;
       s.fine_weight[tid] = 0;
-      if (tid == 0) s.taken = 0;
       __syncthreads();
-#pragma unroll
-      for (int j = 0; j < kEach; ++j) {
-        const uint32_t at = tid + j * kThreads;
-        fine[j] = -1;
-        if (at >= listed) continue;
-        const float x = key_logit(s.keys[i][at]);
-        if (bin_of(w, x) != p.bin) continue;
-        const double y = past_edge(w, x, p.bin), g = y * kThreads;
-        fine[j] = g > 0.0 ? (g < kThreads - 1 ? static_cast<int>(g) : kThreads - 1) : 0;
-        atomicAdd(&s.fine_count[fine[j]], 1u);
-        atomicAdd(&s.fine_weight[fine[j]], static_cast<unsigned long long>(weight_in_bin(y)));
-      }
+      each_listed([&](uint64_t k, float x) {
+        const int d = fine_of(x);
+        atomicAdd(&s.fine_count[d], 1u);
+        atomicAdd(&s.fine_weight[d], static_cast<unsigned long long>(key_weight(w, k, p.bin)));
+      });
       __syncthreads();
       Place q = p;
       narrow(s.ranks, q, b, s.fine_count[tid], s.fine_weight[tid]);
@@ -724,10 +734,11 @@ __global__ __launch_bounds__(kThreads) void sample_pick(SampleArgs a) {
       if (whole) p = q;
     }
     if (whole) {
-#pragma unroll
-      for (int j = 0; j < kEach; ++j)
-        if (fine[j] == only)
-          s.near[atomicAdd(&s.taken, 1u)] = s.keys[i][tid + j * kThreads];
+      if (tid == 0) s.taken = 0;
+      __syncthreads();
+      each_listed([&](uint64_t k, float x) {
+        if (only < 0 || fine_of(x) == only) s.near[atomicAdd(&s.taken, 1u)] = k;
+      });
     } else {
       reread<L>(a, s, w, r, p, b);
     }

@@ -109,6 +109,18 @@ def test_many_tokens_on_few_values():
         check(logits.to(torch.bfloat16), uniforms(k + 1, 12), top_k=k, top_p=0.7)
 
 
+@pytest.mark.parametrize("kind", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("std", [0.1, 0.3, 0.6, 1.2])
+@pytest.mark.parametrize("rows,vocab", [(2, 151936), (5, 40000), (60, 20000)])
+def test_flat_rows_with_thousands_of_tokens_in_a_bin(rows, vocab, std, kind):
+    """A bin, 1/32 nat, of 500 to 19000 tokens: lists in the block, in memory, and rows
+    that are read again."""
+    logits = normal(vocab + rows, rows, vocab, std=std).to(kind)
+    for i, settings in enumerate((dict(), dict(top_p=0.6), dict(temperature=1.5, top_k=vocab // 3, top_p=0.9),
+                                  dict(temperature=0.8, min_p=0.4))):
+        check(logits, uniforms(rows + i, rows), **settings)
+
+
 def test_masked_and_infinite_logits():
     logits = normal(4, 10, 3000, std=2.0)
     logits[0] = -INF
