@@ -21,16 +21,16 @@
 //   4. every chunk: its tokens in these bins as lists;
 //   5. one block a row: each border in turn, its bin and then its tokens, by 1024
 //      finer bins and by rank. Lists of more than 2048 tokens stay in memory; where
-//      a chunk's own passes that, or a finer bin holds more than 1024 tokens (a flat
-//      row, or many equal logits), the bin's tokens are read again from the row,
-//      narrowed by eight bits of (logit, id) at a time.
+//      a chunk's own passes that, the bin's tokens are read again from the row. More
+//      than 1024 in a finer bin (many equal logits) are narrowed by eight bits of
+//      (logit, id) at a time.
 //
-// One row of 151936 bf16 logits takes 27 us: five launches of 3, 5, 6, 4.5 and
-// 10 us, each a chain of loads, scans and barriers. 64 such rows in fp32 (39 MB)
-// take 56: 6.5, 15, 9, 11 and 15 us, the second bound by the 64-bit additions to LDS
-// bins. Steps 2 + 3 and 4 + 5 in one launch each, by the row's last block, save one
-// row 2.5 us and cost 64 rows 12; steps 3 + 4, each block planning for itself, 1.6
-// and 2 to 20.
+// One row of 151936 bf16 logits takes 23.7 us: five launches of 3, 5, 6, 4.5 and
+// 7 us, each a chain of loads, scans and barriers. 64 such rows in fp32 (39 MB) take
+// 51: 6.5, 15, 9, 11 and 10.5 us, the second bound by the 64-bit additions to LDS
+// bins. A row of equal logits takes 165. Before its steps were as short, steps 2 + 3
+// and 4 + 5 in one launch each, by the row's last block, gained one row 0.8 us and
+// cost 64 rows 12; steps 3 + 4, each block planning for itself, gained 1.6 and cost 2.
 #include "common.h"
 
 namespace htn {
@@ -346,25 +346,23 @@ __global__ __launch_bounds__(kThreads) void sample_plan(SampleArgs a) {
   __shared__ uint64_t whole;
   const int tid = threadIdx.x, lane = tid & 63, r = blockIdx.x;
   const long row_at = static_cast<long>(r) * a.chunks;
-  // The row's bins (a thread's own one), and what min-p keeps at its edge.
+  // The row's bins (a thread's own one), and what min-p keeps at its edge: all loads
+  // in flight at once.
+  uint64_t v[kMaxChunks], edge[3];
+#pragma unroll
+  for (int i = 0; i < kMaxChunks; ++i) v[i] = i < a.chunks ? a.bins[(row_at + i) * kBins + tid] : 0;
+#pragma unroll
+  for (int i = 0; i < 3; ++i) edge[i] = lane < a.chunks ? a.edges[(row_at + lane) * 3 + i] : 0;
+  const Row w = row_of(a, r);
+  const Settings set = settings_of(a, w, r);
+  if (w.none) return;
   uint32_t count = 0;
   uint64_t sum = 0;
-  for (int i0 = 0; i0 < a.chunks; i0 += 8) {
-    uint64_t v[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i0 + i < a.chunks ? a.bins[(row_at + i0 + i) * kBins + tid] : 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      count += static_cast<uint32_t>(v[i] >> kCountBit);
-      sum += v[i] & ((1ULL << kCountBit) - 1);
-    }
+  for (int i = 0; i < kMaxChunks; ++i) {
+    count += static_cast<uint32_t>(v[i] >> kCountBit);
+    sum += v[i] & ((1ULL << kCountBit) - 1);
   }
-  const Row w = row_of(a, r);
-  uint64_t edge[3];
-#pragma unroll
-  for (int i = 0; i < 3; ++i) edge[i] = w.cut && lane < a.chunks ? a.edges[(row_at + lane) * 3 + i] : 0;
-  if (w.none) return;
-  const Settings set = settings_of(a, w, r);
   if (tid == 0) whole = 0;
   uint32_t c1 = count;
   uint64_t w1 = outside(sum, unit_of(tid));
@@ -455,7 +453,7 @@ __global__ __launch_bounds__(kThreads) void sample_collect(SampleArgs a) {
   uint64_t* lists = a.lists + at * kBorders * kListed;
   const long from = c * a.chunk;
   if (any_hi >= any_lo)
-    each_logit<L, 4>(static_cast<const L*>(a.logits) + r * a.row_st, from, chunk_end(a, from),
+    each_logit<L, 2>(static_cast<const L*>(a.logits) + r * a.row_st, from, chunk_end(a, from),
                      [&](float x, long id) {
                        x = seen_logit(w, x);
                        const int bin = bin_of(w, x);
@@ -583,48 +581,71 @@ __device__ __forceinline__ Found among_few(Shared& s, const Row& w, uint64_t* ke
   return s.found;
 }
 
-// Narrows a place to 1024 tokens at most, its tokens read from the row again, eight
-// bits of the key at a time, and leaves their keys in `near`.
-template <typename L>
-__device__ __forceinline__ void reread(const SampleArgs& a, Shared& s, const Row& w, int r, Place& p,
-                                       const Border& b) {
+// Narrows a place to 1024 tokens at most, by eight bits of the key at a time from
+// the first in which they differ, and leaves their keys in `near`. each(f) calls
+// f(key) for the tokens of the place's bin.
+template <typename E>
+__device__ __forceinline__ void by_digits(Shared& s, const Row& w, Place& p, const Border& b, E&& each) {
   const int tid = threadIdx.x;
-  const L* row = static_cast<const L*>(a.logits) + r * a.row_st;
-  uint64_t prefix = 0;
-  int bits = 64;
-  // f(key) for the bin's tokens whose key agrees with `prefix` above `bits`.
-  auto each_token = [&](auto&& f) {
-    each_logit<L, 4>(row, 0, a.vocab, [&](float x, long id) {
-      x = seen_logit(w, x);
-      if (bin_of(w, x) != p.bin) return;
-      const uint64_t key = order_key(x, id);
+  enum { kCommon, kDigits, kGather } step = kCommon;
+  uint64_t all = ~0ULL, prefix = 0;
+  int bits = 64, digit = 0;  // keys sought agree with the prefix above `bits`
+#pragma unroll 1
+  for (;;) {
+    __syncthreads();
+    if (step == kDigits) {
+      s.fine_count[tid] = 0;
+      s.fine_weight[tid] = 0;
+    } else if (tid == 0) {
+      s.taken = 0;
+      s.near[0] = ~0ULL;
+      s.near[1] = 0;
+    }
+    __syncthreads();
+    each([&](uint64_t key) {
+      if (step == kCommon) {
+        all &= key;
+        prefix |= key;
+        return;
+      }
       if (bits < 64 && (key ^ prefix) >> bits) return;
-      f(key);
+      if (step == kDigits) {
+        // Larger keys first; four sums a digit, as neighbours tend to share it.
+        const int d = 4 * (255 - static_cast<int>((key >> (bits - digit)) & ((1 << digit) - 1))) + (tid & 3);
+        atomicAdd(&s.fine_count[d], 1u);
+        atomicAdd(&s.fine_weight[d], static_cast<unsigned long long>(key_weight(w, key, p.bin)));
+      } else {
+        const uint32_t i = atomicAdd(&s.taken, 1u);
+        if (i < kThreads) s.near[i] = key;
+      }
     });
-  };
-  while (p.here > kThreads) {  // keys differ, so eight digits at most
-    __syncthreads();
-    s.fine_count[tid] = 0;
-    s.fine_weight[tid] = 0;
-    __syncthreads();
-    each_token([&](uint64_t key) {
-      const int d = 255 - static_cast<int>((key >> (bits - 8)) & 255);  // larger keys first
-      atomicAdd(&s.fine_count[d], 1u);
-      atomicAdd(&s.fine_weight[d], static_cast<unsigned long long>(key_weight(w, key, p.bin)));
-    });
-    __syncthreads();
-    narrow(s.ranks, p, b, s.fine_count[tid], s.fine_weight[tid]);
-    bits -= 8;
-    prefix = (prefix & (bits < 56 ? ~0ULL << (bits + 8) : 0ULL)) |
-             (static_cast<uint64_t>(255 - s.ranks.at) << bits);
+    if (step == kGather) return;
+    if (step == kCommon) {
+      atomicAnd(reinterpret_cast<unsigned long long*>(&s.near[0]), static_cast<unsigned long long>(all));
+      atomicOr(reinterpret_cast<unsigned long long*>(&s.near[1]), static_cast<unsigned long long>(prefix));
+      __syncthreads();
+      prefix = s.near[1];
+      const uint64_t differ = prefix & ~s.near[0];
+      bits = differ ? 64 - __builtin_clzll(differ) : 0;
+      prefix = bits < 64 ? prefix >> bits << bits : 0;
+    } else {
+      __syncthreads();
+      uint32_t count = 0;
+      uint64_t sum = 0;
+      if (tid < 256) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          count += s.fine_count[4 * tid + i];
+          sum += s.fine_weight[4 * tid + i];
+        }
+      }
+      narrow(s.ranks, p, b, count, sum);
+      bits -= digit;
+      prefix |= static_cast<uint64_t>(255 - s.ranks.at) << bits;
+    }
+    step = p.here > kThreads && bits > 0 ? kDigits : kGather;
+    digit = bits < 8 ? bits : 8;
   }
-  __syncthreads();
-  if (tid == 0) s.taken = 0;
-  __syncthreads();
-  each_token([&](uint64_t key) {
-    const uint32_t i = atomicAdd(&s.taken, 1u);
-    if (i < kThreads) s.near[i] = key;
-  });
 }
 
 template <typename L>
@@ -696,17 +717,17 @@ __global__ __launch_bounds__(kThreads) void sample_pick(SampleArgs a) {
         if (bin_of(w, x) == p.bin) g(k, x);
       };
       if (listed <= kListed) {
-#pragma unroll
+#pragma unroll 1
         for (int j = 0; j < kEach; ++j)
           if (tid + j * kThreads < listed) one(s.keys[i][tid + j * kThreads]);
         return;
       }
-      for (uint32_t at = tid; at < listed; at += 4 * kThreads) {
-        uint64_t k[4];
+      for (uint32_t at = tid; at < listed; at += 2 * kThreads) {
+        uint64_t k[2];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) k[u] = key_at(i, at + u * kThreads < listed ? at + u * kThreads : at);
+        for (int u = 0; u < 2; ++u) k[u] = key_at(i, at + u * kThreads < listed ? at + u * kThreads : at);
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
+        for (int u = 0; u < 2; ++u)
           if (at + u * kThreads < listed) one(k[u]);
       }
     };
@@ -740,7 +761,16 @@ __global__ __launch_bounds__(kThreads) void sample_pick(SampleArgs a) {
         if (only < 0 || fine_of(x) == only) s.near[atomicAdd(&s.taken, 1u)] = k;
       });
     } else {
-      reread<L>(a, s, w, r, p, b);
+      by_digits(s, w, p, b, [&](auto&& g) {
+        if (listed) {
+          each_listed([&](uint64_t k, float) { g(k); });
+          return;
+        }
+        each_logit<L, 1>(static_cast<const L*>(a.logits) + r * a.row_st, 0, a.vocab, [&](float x, long id) {
+          x = seen_logit(w, x);
+          if (bin_of(w, x) == p.bin) g(order_key(x, id));
+        });
+      });
     }
     f = p.here <= kWave ? among_few(s, w, s.near, p, b) : among(s, w, s.near, p, b);
     kept = i < 2 ? least(kept, f.weight) : kept;

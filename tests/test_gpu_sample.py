@@ -121,6 +121,18 @@ def test_flat_rows_with_thousands_of_tokens_in_a_bin(rows, vocab, std, kind):
         check(logits, uniforms(rows + i, rows), **settings)
 
 
+@pytest.mark.parametrize("vocab,tie", [(151936, 2500), (151936, 1030), (20000, 19000), (40000, 1025)])
+def test_thousands_of_equal_logits_inside_a_row(vocab, tie):
+    """As coarse logits have them: `tie` tokens on one value, in the lists or past them."""
+    g = torch.Generator().manual_seed(tie)
+    logits = torch.randn(4, vocab, generator=g) * 2 + 20
+    for r in range(4):
+        logits[r, torch.randperm(vocab, generator=g)[:tie]] = 20.125 + r
+    for settings in (dict(), dict(temperature=2.0), dict(top_p=0.5), dict(top_k=tie // 2, temperature=30.0)):
+        check(logits, uniforms(tie, 4), **settings)
+        check(logits.to(torch.bfloat16), uniforms(vocab, 4), **settings)
+
+
 def test_masked_and_infinite_logits():
     logits = normal(4, 10, 3000, std=2.0)
     logits[0] = -INF
