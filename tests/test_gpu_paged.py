@@ -379,6 +379,20 @@ def test_captured_decode_step_replays_with_other_lengths(new):
                 assert torch.equal(got, eager)
 
 
+@pytest.mark.parametrize("new,length", [(5, 900), (64, 2000), (200, 700)])
+def test_rows_do_not_depend_on_other_rows_scores(new, length):
+    """Every other token's queries 20 times as large (their maxima move far more often):
+    the others' outputs stay the same, bit for bit."""
+    b = Batch([new], [length], 4, 4, 16)
+    b.q *= 3
+    q, *rest = b.cuda()
+    want = paged_attention(q, *rest)
+    q[1::2] *= 20
+    got = paged_attention(q, *rest)
+    assert torch.equal(got[::2], want[::2])
+    assert not torch.equal(got[1::2], want[1::2])
+
+
 def test_calls_repeat_bit_for_bit():
     b = Batch([1, 90, 1], [3000, 900, 77], 32, 8, 16)
     args = b.cuda()
