@@ -488,6 +488,17 @@ __device__ __forceinline__ float max3(float x, float y, float z) {
   return r;
 }
 
+// quad_max of a value that max3 made.
+__device__ __forceinline__ float quad_max3(float v) {
+  auto pair = [](auto w) {
+    float r;
+    asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(__uint_as_float(w[0])), "v"(__uint_as_float(w[1])));
+    return r;
+  };
+  v = pair(__builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+  return pair(__builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+}
+
 // The wait states that a vector instruction must keep from the matrix instruction
 // whose result it reads (19 at most), which the compiler does not insert ahead of
 // inline asm.
@@ -821,7 +832,7 @@ __device__ __forceinline__ void attend_many(const PagedArgs& a, const Item& it, 
 #pragma unroll
       for (int i = 3; i < 15; i += 2)
         tmax = max3(tmax, st[n][i / 4][i % 4], st[n][(i + 1) / 4][(i + 1) % 4]);
-      tmax = quad_max(fmaxf(tmax, st[n][3][3]));
+      tmax = quad_max3(max3(tmax, st[n][3][3], st[n][3][3]));
       const bool moves = tmax > m[n] + slack;  // see kSlack
       if (__builtin_expect(__any(moves), 0)) {
         const float m_new = moves ? tmax : m[n];  // of that row alone: no row's sums depend on another's scores
