@@ -346,21 +346,23 @@ __device__ __forceinline__ bool make_plan(const PagedArgs& a, int prefix, Item& 
   return found;
 }
 
-// Where a 16-slot group's K or V rows lie in a pool: an element offset, and the
-// rows that may be read (the rest of the group reads as zeros).
+// The page of the 16-slot group at `slot`, -1 where none of slots lo0 .. hi - 1 is in it.
+__device__ __forceinline__ int page_of(const PagedArgs& a, const int32_t* table, int slot, int lo0, int hi) {
+  return slot < hi && slot + 16 > lo0 ? scalar_i32(table, slot >> a.page_shift) : -1;
+}
+
+// Where a group's K or V rows lie in a pool: an element offset, and the rows that may
+// be read (the rest of the group reads as zeros).
 struct Group {
   long offset;
   uint32_t bytes;
 };
 
-__device__ __forceinline__ Group group_of(const PagedArgs& a, const int32_t* table, int kvh, int slot,
-                                          int lo0, int hi) {
-  const bool some = slot < hi && slot + 16 > lo0;
-  const int id = some ? scalar_i32(table, slot >> a.page_shift) : -1;
-  const bool in_pool = id >= 0 && id < a.pages;
+__device__ __forceinline__ Group group_of(const PagedArgs& a, int page, int kvh, int slot, int hi) {
+  const bool in_pool = page >= 0 && page < a.pages;
   const int left = hi - slot;
   Group g;
-  g.offset = in_pool ? ((((static_cast<long>(id) * a.Hkv + kvh) << a.page_shift) +
+  g.offset = in_pool ? ((((static_cast<long>(page) * a.Hkv + kvh) << a.page_shift) +
                          (slot & ((1 << a.page_shift) - 1))) * D) : 0;
   g.bytes = in_pool ? static_cast<uint32_t>(left < 16 ? left : 16) * (D * 2) : 0u;
   return g;
@@ -378,19 +380,13 @@ __device__ __forceinline__ void stage_offsets(int lane, uint32_t (&off)[2]) {
   }
 }
 
-// This wave's 16 slots of a tile, K then V, by eight 1 KB LDS-direct loads.
-__device__ __forceinline__ void stage_group(const PagedArgs& a, const Group& g, unsigned char* k_lds,
-                                            unsigned char* v_lds, const uint32_t (&off)[2]) {
-  const __amdgpu_buffer_rsrc_t krs = uniform_rsrc(a.keys + g.offset, g.bytes);
-  const __amdgpu_buffer_rsrc_t vrs = uniform_rsrc(a.values + g.offset, g.bytes);
-#pragma unroll
-  for (int u = 0; u < 4; ++u)
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(krs, (lds_void_t*)(k_lds + u * 1024), 16, off[u & 1] + (u >> 1) * 2048,
-                                             0, 0, 0);
-#pragma unroll
-  for (int u = 0; u < 4; ++u)
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(vrs, (lds_void_t*)(v_lds + u * 1024), 16, off[u & 1] + (u >> 1) * 2048,
-                                             0, 0, 0);
+// Quarter u of a group's K or V rows, a 1 KB LDS-direct load (whose own offset moves
+// both ends).
+__device__ __forceinline__ void stage_quarter(__amdgpu_buffer_rsrc_t rows, unsigned char* lds, int u,
+                                              const uint32_t (&off)[2]) {
+  lds_void_t* to = (lds_void_t*)(lds + (u & 1) * 1024);
+  if (u & 2) __builtin_amdgcn_raw_ptr_buffer_load_lds(rows, to, 16, off[u & 1], 0, 2048, 0);
+  else __builtin_amdgcn_raw_ptr_buffer_load_lds(rows, to, 16, off[u & 1], 0, 0, 0);
 }
 
 // Addresses of the operand reads in a tile whose K rows start at LDS byte k and V
@@ -478,6 +474,12 @@ __device__ __forceinline__ void add_nonfinite(const unsigned char* v, int slots,
 __device__ __forceinline__ f32x4_t mfma(u32x4 x, u32x4 y, f32x4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, x),
                                                  __builtin_bit_cast(bf16x8_t, y), c, 0, 0, 0);
+}
+
+// Until at most N of the wave's LDS reads are left, after which these are there.
+template <int N>
+__device__ __forceinline__ void wait_k4(u32x4 (&k)[4]) {
+  asm volatile("s_waitcnt lgkmcnt(%4)" : "+v"(k[0]), "+v"(k[1]), "+v"(k[2]), "+v"(k[3]) : "n"(N) : "memory");
 }
 
 // The largest of three; fmaxf first quiets each operand, an instruction of its own.
@@ -584,9 +586,14 @@ __device__ __forceinline__ void attend_few(const PagedArgs& a, const Item& it, c
   // count of loads in flight stays the same.
   auto stage = [&](int i) {
     Group g{0, 0};
-    if (i < i1) g = group_of(a, table, it.kvh, slot_of(i), sl.lo0, sl.hi);
+    if (i < i1) g = group_of(a, page_of(a, table, slot_of(i), sl.lo0, sl.hi), it.kvh, slot_of(i), sl.hi);
+    const __amdgpu_buffer_rsrc_t k_rows = uniform_rsrc(a.keys + g.offset, g.bytes);
+    const __amdgpu_buffer_rsrc_t v_rows = uniform_rsrc(a.values + g.offset, g.bytes);
     unsigned char* b = lds + ((i - i0) % kRing) * kTileBytes;
-    stage_group(a, g, b, b + kGroupBytes, off);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) stage_quarter(k_rows, b, u, off);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) stage_quarter(v_rows, b + kGroupBytes, u, off);
   };
   __builtin_amdgcn_sched_barrier(0);
   if (i0 < i1) {
@@ -747,7 +754,7 @@ __device__ __forceinline__ void attend_many(const PagedArgs& a, const Item& it, 
   const int sinks = a.window ? a.sinks : 0;
   u32x4 qf[2][4];
   Sight sight[2];
-  int all_hi = 0x7fffffff, all_lo = -0x7fffffff, any_hi = -1, any_lo = 0x7fffffff;
+  int all_hi = 0x7fffffff, all_lo = -0x7fffffff;
 #pragma unroll
   for (int n = 0; n < 2; ++n) {
     const int r = 32 * wave + 16 * n + col;
@@ -759,24 +766,40 @@ __device__ __forceinline__ void attend_many(const PagedArgs& a, const Item& it, 
     const int first = it.t0 + it.tile * kManyRows / a.G;
     sight[n] = sight_of(it.seq < 0 ? rowpos[t - first] : it.p0 + (t - it.t0), sl, a.window);
     const int lo = min16(sight[n].vhi), hi = -min16(-sight[n].vlo);
-    const int top = -min16(-sight[n].vhi), low = min16(sight[n].vlo);
     all_hi = lo < all_hi ? lo : all_hi;
     all_lo = hi > all_lo ? hi : all_lo;
-    any_hi = top > any_hi ? top : any_hi;
-    any_lo = low < any_lo ? low : any_lo;
   }
   uint32_t off[2];
   stage_offsets(lane, off);
   auto tile_of = [&](int i) {
     return (i < sl.sink_tiles ? i : i - sl.sink_tiles + sl.first_tile) * kSplit;
   };
-  auto stage = [&](int i) {
-    const Group g = group_of(a, table, it.kvh, tile_of(i) + wave * 16, sl.lo0, sl.hi);
+  // A tile is staged during the work on the one before, 16 slots a wave, a load after
+  // every four products (all eight at once hold the wave), from descriptors made a
+  // tile and a page looked up two tiles ahead. Past the last tile they load zeros.
+  auto page_at = [&](int i) {
+    return i < i1 ? page_of(a, table, tile_of(i) + wave * 16, sl.lo0, sl.hi) : -1;
+  };
+  int page = page_at(i0);
+  __amdgpu_buffer_rsrc_t k_rows, v_rows;
+  auto prepare = [&](int i) {
+    const Group g = group_of(a, page, it.kvh, tile_of(i) + wave * 16, sl.hi);
+    k_rows = uniform_rsrc(a.keys + g.offset, g.bytes);
+    v_rows = uniform_rsrc(a.values + g.offset, g.bytes);
+    page = page_at(i + 1);
+  };
+  auto load = [&](int i, int u) {
     unsigned char* b = ring + ((i - i0) & 1) * kTileBytes + wave * kGroupBytes;
-    stage_group(a, g, b, b + kSplit * D * 2, off);
+    if (u < 4) stage_quarter(k_rows, b, u, off);
+    else stage_quarter(v_rows, b + kSplit * D * 2, u - 4, off);
   };
   __builtin_amdgcn_sched_barrier(0);
-  if (i0 < i1) stage(i0);
+  if (i0 < i1) {
+    prepare(i0);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) load(i0, u);
+    prepare(i0 + 1);
+  }
   const uint32_t ring_base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void_t*)ring));
   const ReadAddrs from = read_addrs(ring_base, ring_base + kSplit * D * 2, col, quad);
   const u32x4 ones = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
@@ -789,24 +812,28 @@ __device__ __forceinline__ void attend_many(const PagedArgs& a, const Item& it, 
 #pragma unroll
     for (int j = 0; j < 8; ++j) acc[n][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
-  auto tile = [&](int s0, uint32_t tb, bool whole) {
+  auto tile = [&](int i, int s0, uint32_t tb, bool whole) {
     f32x4_t st[2][4];
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int mt = 0; mt < 4; ++mt) st[n][mt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     u32x4 kf[4][4];
     issue_k_pf<0>(k_addr(from, 0, tb), kf[0]);
     issue_k_pf<0>(k_addr(from, 1, tb), kf[1]);
     issue_k_pf<0>(k_addr(from, 2, tb), kf[2]);
     issue_k_pf<0>(k_addr(from, 3, tb), kf[3]);
-    wait_k16(kf);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int ks = 0; ks < 4; ++ks)
+      for (int ks = 0; ks < 4; ++ks) {
+        if (n == 0 && ks == 0) wait_k4<12>(kf[0]);  // K as it arrives
+        if (n == 0 && ks == 1) wait_k4<8>(kf[1]);
+        if (n == 0 && ks == 2) wait_k4<4>(kf[2]);
+        if (n == 0 && ks == 3) wait_k4<0>(kf[3]);
 #pragma unroll
-        for (int mt = 0; mt < 4; ++mt) st[n][mt] = mfma(kf[ks][mt], qf[n][ks], st[n][mt]);
+        for (int mt = 0; mt < 4; ++mt)
+          st[n][mt] = mfma(kf[ks][mt], qf[n][ks], ks ? st[n][mt] : f32x4_t{0.f, 0.f, 0.f, 0.f});
+        load(i + 1, 4 * n + ks);
+        __builtin_amdgcn_sched_barrier(0);
+      }
     // The V^T operands of half the tile in flight during the softmax.
     uint32_t va[8];
 #pragma unroll
@@ -844,10 +871,13 @@ __device__ __forceinline__ void attend_many(const PagedArgs& a, const Item& it, 
         m[n] = m_new;
         base[n] = ms;
       }
-      // Keeps the accumulators in place: the branch not taken copied them (mixed batch
-      // 127 -> 123 us).
+      // The branch not taken would copy the accumulators into the products' registers:
+      // they pass into another block first.
 #pragma unroll
       for (int j = 0; j < 8; ++j) asm volatile("" : "+v"(acc[n][j]));
+      int never = 0;
+      asm volatile("" : "+s"(never));
+      if (__builtin_expect(never, 0)) asm volatile("s_nop 0");
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) {
         float p[4];
@@ -934,9 +964,8 @@ __device__ __forceinline__ void attend_many(const PagedArgs& a, const Item& it, 
         __syncthreads();
       }
     }
-    if (i + 1 < i1) stage(i + 1);
-    if (active && s0 <= any_hi && (s0 + kSplit > any_lo || s0 < sinks))
-      tile(s0, tb, seen_by_all(s0, all_hi, all_lo));
+    tile(i, s0, tb, seen_by_all(s0, all_hi, all_lo));
+    prepare(i + 2);
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   const late_args_t la = late_args();
