@@ -736,12 +736,14 @@ __device__ __forceinline__ void attend_few(const PagedArgs& a, const Item& it, c
 // row's weights add up to 1.
 //
 // Bound by the matrix and vector instructions, which share a SIMD's issue: a
-// 5000-token prompt of 32 + 8 heads takes 240-250 us, 0.82-0.85 PFLOP/s of the
-// causal products (an 8192^3 product 1.35), with the matrix cores at work in 41% of
-// the cycles and vector instructions issued in 37%; LDS reads take a quarter.
-// Neither 32x32 products, nor loads spread between the products, nor one half's
-// products under the other half's softmax, nor fewer vector instructions (weights
-// cut instead of rounded) changed that by more than 2%.
+// 5000-token prompt of 32 + 8 heads takes 228-235 us, 0.87-0.9 PFLOP/s of the causal
+// products (an 8192^3 product 1.35), with the matrix cores at work in 44% of the
+// cycles and vector instructions issued in 33%; LDS reads take a quarter. Neither
+// 32x32 products, nor one half's products under the other half's softmax, nor fewer
+// vector instructions (weights cut instead of rounded) changed that by more than 2%.
+// A 1000-token chunk beside 15 single tokens, where a block has half a CU's issue to
+// itself, takes 109-114 us, 0.53 PFLOP/s; staging loads all at the start of a tile,
+// waiting for all of K, and accumulators copied around the rescaling made that 121.
 __device__ __forceinline__ void attend_many(const PagedArgs& a, const Item& it, const Slots& sl,
                                             const int32_t* table, const int* rowpos,
                                             unsigned char* ring, int2* bounds, int* odd_tile) {
