@@ -260,6 +260,59 @@ def test_shared_prefix_matches_plain(new, lengths, heads, kv_heads, page, prefix
     b.check(none)
 
 
+@pytest.mark.parametrize("seed", range(16))
+def test_drawn_batches_match_plain(seed):
+    """Batches of 1 to 150 sequences with none, one, a few or many new tokens each, groups
+    of 1 to 160 heads, all page sizes, windows and prefixes as they come."""
+    g = torch.Generator().manual_seed(100 + seed)
+
+    def draw(options):
+        return options[int(torch.randint(len(options), (1,), generator=g))]
+    heads, kv_heads = draw([(160, 1), (33, 1), (48, 4), (7, 7), (32, 8), (4, 2), (130, 2)])
+    page, count = draw([16, 32, 64, 256, 1024]), draw([1, 2, 5, 64, 65, 150])
+    most = 600 if count <= 5 else 60
+    new = [draw([0, 1, 1, 1, 3, 9, most // 2, most]) if count <= 5 or draw([0, 1]) else 1
+           for _ in range(count)]
+    new[draw(range(count))] = 1
+    prefix = draw([0, 0, 16, 50, 300])
+    lengths = [prefix + n + draw([0, 0, 1, 40, most]) for n in new]
+    b = Batch(new, lengths, heads, kv_heads, page, seed=seed, prefix=prefix // page * page)
+    args = b.cuda()
+    window, sinks = draw([(0, 0), (1, 0), (37, 5), (200, 64)])
+    b.check(paged_attention(*args, window=window, sinks=sinks), window, sinks)
+    if prefix // page:
+        q, keys, values, table, starts, dev_lengths = args
+        whole = prefix // page
+        b.check(shared_prefix_attention(q, keys, values, table[0, :whole].contiguous(),
+                                        torch.tensor([whole * page], device="cuda"), table, starts,
+                                        dev_lengths))
+
+
+def test_two_graphs_replayed_in_turn():
+    """Calls of two captured graphs keep workspaces of their own."""
+    batches = [Batch([1, 20, 3], [900, 300, 500], 16, 4, 16, seed=1), Batch([60, 1], [700, 2000], 8, 8, 64, seed=2)]
+    graphs, outs, wants = [], [], []
+    for b in batches:
+        args = b.cuda()
+        wants.append(paged_attention(*args))
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            paged_attention(*args)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            outs.append(paged_attention(*args))
+        graphs.append((graph, args))
+    for _ in range(3):
+        for graph, _ in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for out, want in zip(outs, wants):
+            assert torch.equal(out, want)
+            out.zero_()
+
+
 def test_prefix_past_a_rows_position_stays_causal():
     """Rows inside the prefix see it only up to themselves."""
     b = Batch([100, 3], [180, 150], 8, 4, 16, prefix=128)
