@@ -1039,18 +1039,18 @@ __global__ __launch_bounds__(kBlock, 2) void paged_attention_kernel(PagedArgs a)
 // 4-6 us, 2048 blocks at most; one that finds nothing split ends at once.
 __global__ __launch_bounds__(kBlock) void paged_merge_kernel(PagedArgs a) {
   const int lane = threadIdx.x & 63, half = lane >> 5, dim = 4 * (lane & 31);
-  if (!a.plan[0].split) return;
+  const int split = a.plan[0].split;
   const bool shared = a.prefix_length != nullptr;
   const long rows = static_cast<long>(a.T) * a.Hq;
   for (long orow = static_cast<long>(blockIdx.x) * 4 + (threadIdx.x >> 6); orow < rows;
        orow += static_cast<long>(gridDim.x) * 4) {
     const int t = static_cast<int>(orow / a.Hq), h = static_cast<int>(orow % a.Hq);
     const int j = sequence_of(a.starts, a.B, t, lane);
+    if (!split) return;
     if (j >= a.B) continue;
     const PlanEntry own = a.plan[j + (shared ? 1 : 0)];
-    if (!own.chunks) continue;
-    const Span s = make_span(a.starts[j], a.starts[j + 1], a.lengths[j], a.T, a.table_pages << a.page_shift);
-    if (t < s.t0 || t >= s.t0 + s.n) continue;
+    const int64_t from = a.starts[j], to = a.starts[j + 1], end = a.starts[a.B];
+    if (!own.chunks || t < from || t >= to) continue;  // with chunks, starts rise
     const int kvh = h / a.G;
     float M = -INFINITY, L = 0.f;
     f32x4_t o = {0.f, 0.f, 0.f, 0.f};
@@ -1062,6 +1062,16 @@ __global__ __launch_bounds__(kBlock) void paged_merge_kernel(PagedArgs a) {
       for (int c0 = 0; c0 < p.chunks; c0 += kWave) {
         const int n = p.chunks - c0 < kWave ? p.chunks - c0 : kWave;
         const float2 ml = lane < n ? a.ml[row + (c0 + lane) * step] : make_float2(-INFINITY, 0.f);
+        constexpr int U = 8;
+        f32x4_t x[U];
+        auto fetch = [&](int c) {
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const int at = c + 2 * u + half;
+            x[u] = *reinterpret_cast<const f32x4_t*>(a.part + (row + (c0 + (at < n ? at : 0)) * step) * D + dim);
+          }
+        };
+        fetch(0);
         const float mb = fmaxf(M, wave_max(ml.x));
         if (mb == -INFINITY) continue;
         const float f0 = share(M - mb);
@@ -1069,25 +1079,21 @@ __global__ __launch_bounds__(kBlock) void paged_merge_kernel(PagedArgs a) {
         M = mb;
         L = fmaf(L, f0, wave_sum(f * ml.y));
         o *= f0;
-        constexpr int U = 8;
-        for (int c = 0; c < n; c += 2 * U) {
-          f32x4_t x[U];
-          float g[U];
+        for (int c = 0;;) {
 #pragma unroll
           for (int u = 0; u < U; ++u) {
-            const int at = c + 2 * u + half, k = at < n ? at : 0;
-            x[u] = *reinterpret_cast<const f32x4_t*>(a.part + (row + (c0 + k) * step) * D + dim);
-            const float fk = __shfl(f, k, kWave);
-            g[u] = at < n ? fk : 0.f;
+            const int at = c + 2 * u + half;
+            const float g = __shfl(f, at < n ? at : 0, kWave);
+            if (at < n && g != 0.f) o += x[u] * g;  // a chunk that saw nothing wrote no weights
           }
-#pragma unroll
-          for (int u = 0; u < U; ++u)
-            if (g[u] != 0.f) o += x[u] * g[u];  // a chunk that saw nothing wrote no weights
+          c += 2 * U;
+          if (c >= n) break;
+          fetch(c);
         }
       }
     };
-    fold(own, t - s.t0, s.n);
-    if (shared) fold(a.plan[0], t, static_cast<int>(a.starts[a.B]));
+    fold(own, t - static_cast<int>(from), static_cast<int>(to - from));
+    if (shared) fold(a.plan[0], t, static_cast<int>(end));
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], 32, kWave);
     const float inv = M == -INFINITY ? 0.f : 1.0f / L;
