@@ -170,7 +170,6 @@ struct PagedArgs {
   PlanEntry* plan; float2* ml; float* part;
   int B, T, Hq, Hkv, G;
   int window, sinks;  // window 0: none
-  int target;         // blocks wanted
   float scale2;       // log2(e) / sqrt(128)
 };
 
@@ -242,6 +241,10 @@ __device__ __forceinline__ SeqWork seq_work(const PagedArgs& a, int s, int prefi
   return w;
 }
 
+// Blocks wanted: two per CU, all at once. With 768, 16 sequences (24 K slots) take 28.5 us instead
+// of 25.9, and a 1000-token chunk beside 15 sequences 145 instead of 124.
+constexpr int kTargetBlocks = 512;
+
 // Tiles that a block takes at least, where a row's slots are split: a split
 // writes and merges a partial of its rows (520 bytes each) for K and V of 32 KB
 // a tile. With 1 and with 4, 540 slots under 16 heads take 9.9 and 11.3 us (2:
@@ -268,14 +271,14 @@ struct Item {
 
 // Which rows, K/V head and slots this block takes; false if none. Every wave
 // derives the same plan from starts and lengths, a sequence a lane: the tiles of
-// all rows over `target` blocks give the tiles per block, each sequence's rows are
+// all rows over kTargetBlocks give the tiles per block, each sequence's rows are
 // cut in equal chunks of at most that many, and blocks are numbered sequence by
 // sequence, in each by row tile (the last, longest, first), chunk and K/V head.
 //
 // A sequence's chunks number below twice its tiles over the tiles per block where
-// they are two or more, so all split blocks number below 2 target, and all blocks
-// at most target plus one per (row tile, K/V head). With 64 sequences or fewer the
-// tiles per block are raised until all blocks fit `target` (they run at once).
+// they are two or more, so all split blocks number below 2 kTargetBlocks, and all blocks
+// at most kTargetBlocks plus one per (row tile, K/V head). With 64 sequences or fewer the
+// tiles per block are raised until all blocks fit it (they run at once).
 __device__ __forceinline__ bool make_plan(const PagedArgs& a, int prefix, Item& it) {
   const int lane = threadIdx.x & 63;
   const bool shared = a.prefix_length != nullptr;
@@ -297,12 +300,12 @@ __device__ __forceinline__ bool make_plan(const PagedArgs& a, int prefix, Item& 
   }
   total = wave_last(wave_scan(total));
   items = wave_last(wave_scan(static_cast<uint32_t>(items)));
-  uint32_t per_block = static_cast<uint32_t>((total + a.target - 1) / a.target);
+  uint32_t per_block = static_cast<uint32_t>((total + kTargetBlocks - 1) / kTargetBlocks);
   per_block = per_block > kMinTiles ? per_block : kMinTiles;
-  if (n <= kWave && items <= a.target)
+  if (n <= kWave && items <= kTargetBlocks)
     for (;; per_block += 1 + per_block / 16) {
       const uint32_t mine = lane < n ? w.row_tiles * chunks_of(w, per_block) * a.Hkv : 0;
-      if (wave_last(wave_scan(mine)) <= static_cast<uint32_t>(a.target)) break;
+      if (wave_last(wave_scan(mine)) <= static_cast<uint32_t>(kTargetBlocks)) break;
     }
   // Blocks (low half) and rows of partials (high half) before each sequence.
   uint64_t base = 0;
@@ -510,6 +513,12 @@ __device__ __forceinline__ void settle(f32x4_t (&s)[2][4]) {
                  "+v"(s[1][2]), "+v"(s[1][3]));
 }
 
+// The first of `tiles` tiles that chunk c of n takes: all take the same, some one more.
+__device__ __forceinline__ int chunk_start(int tiles, int c, int n) {
+  const int each = static_cast<uint32_t>(tiles) / static_cast<uint32_t>(n), more = tiles - each * n;
+  return c * each + (c < more ? c : more);
+}
+
 // Token and head of row r of an item's row tile.
 __device__ __forceinline__ void row_of(int group, const Item& it, int tile_rows, int r, int& t, int& h) {
   const int rr = it.tile * tile_rows + r;
@@ -557,8 +566,7 @@ __device__ __forceinline__ void attend_few(const PagedArgs& a, const Item& it, c
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, quad = lane >> 4;
-  const int i0 = static_cast<int>(static_cast<long>(sl.tiles) * it.chunk / it.chunks);
-  const int i1 = static_cast<int>(static_cast<long>(sl.tiles) * (it.chunk + 1) / it.chunks);
+  const int i0 = chunk_start(sl.tiles, it.chunk, it.chunks), i1 = chunk_start(sl.tiles, it.chunk + 1, it.chunks);
   const int sinks = a.window ? a.sinks : 0;
   u32x4 qf[NT][4];
   Sight sight[NT];
@@ -750,8 +758,7 @@ __device__ __forceinline__ void attend_many(const PagedArgs& a, const Item& it, 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, quad = lane >> 4;
-  const int i0 = static_cast<int>(static_cast<long>(sl.tiles) * it.chunk / it.chunks);
-  const int i1 = static_cast<int>(static_cast<long>(sl.tiles) * (it.chunk + 1) / it.chunks);
+  const int i0 = chunk_start(sl.tiles, it.chunk, it.chunks), i1 = chunk_start(sl.tiles, it.chunk + 1, it.chunks);
   const bool active = 32 * wave < it.rows;  // wave-uniform
   const int sinks = a.window ? a.sinks : 0;
   u32x4 qf[2][4];
@@ -1105,9 +1112,6 @@ __global__ __launch_bounds__(kBlock) void paged_merge_kernel(PagedArgs a) {
 
 // ------------------------------------------------------------------ host
 
-// Two per CU, all at once. With 768, 16 sequences (24 K slots) take 28.5 us instead
-// of 25.9, and a 1000-token chunk beside 15 sequences 145 instead of 124.
-constexpr int kTargetBlocks = 512;
 constexpr long kMergeBlocks = 2048;
 constexpr long kMaxSlots = 1L << 29;
 
@@ -1152,7 +1156,6 @@ int attend(PagedArgs& a, void* scratch, int64_t scratch_bytes, hipStream_t st) {
   a.plan = reinterpret_cast<PlanEntry*>(p);
   a.part = reinterpret_cast<float*>(p + s.plan);
   a.ml = reinterpret_cast<float2*>(p + s.plan + s.rows * D * 4);
-  a.target = kTargetBlocks;
   a.scale2 = 1.4426950408889634f / sqrtf(static_cast<float>(D));
   constexpr int lds = kRing * kTileBytes;
   const long merge = (static_cast<long>(a.T) * a.Hq + 3) / 4;
