@@ -241,8 +241,9 @@ __device__ __forceinline__ SeqWork seq_work(const PagedArgs& a, int s, int prefi
   return w;
 }
 
-// Blocks wanted: two per CU, all at once. With 768, 16 sequences (24 K slots) take 28.5 us instead
-// of 25.9, and a 1000-token chunk beside 15 sequences 145 instead of 124.
+// Blocks wanted: two per CU, all at once. With 768, 16 sequences (24 K slots) took
+// 28.5 us instead of 25.9, and a 1000-token chunk beside 15 sequences 145 instead
+// of 124.
 constexpr int kTargetBlocks = 512;
 
 // Tiles that a block takes at least, where a row's slots are split: a split
@@ -276,9 +277,9 @@ struct Item {
 // sequence, in each by row tile (the last, longest, first), chunk and K/V head.
 //
 // A sequence's chunks number below twice its tiles over the tiles per block where
-// they are two or more, so all split blocks number below 2 kTargetBlocks, and all blocks
-// at most kTargetBlocks plus one per (row tile, K/V head). With 64 sequences or fewer the
-// tiles per block are raised until all blocks fit it (they run at once).
+// they are two or more, so all split blocks number below 2 kTargetBlocks, and all
+// blocks at most kTargetBlocks plus one per (row tile, K/V head). With 64 sequences or
+// fewer the tiles per block are raised until all blocks fit it (they run at once).
 __device__ __forceinline__ bool make_plan(const PagedArgs& a, int prefix, Item& it) {
   const int lane = threadIdx.x & 63;
   const bool shared = a.prefix_length != nullptr;
