@@ -203,10 +203,14 @@ struct SeqWork {
   int rows, tile_rows, row_tiles, max_tiles;
 };
 
+// The slots of the shared prefix: of its whole pages. A page that the prefix ends in
+// holds each sequence's own slots behind it, so it is a page of the sequence's, as
+// its table has it.
 __device__ __forceinline__ int prefix_slots(const PagedArgs& a) {
   if (!a.prefix_length) return 0;
   const int64_t p = a.prefix_length[0], cap = a.prefix_count << a.page_shift;
-  return static_cast<int>(p < 0 ? 0 : (p > cap ? cap : p));
+  const int within = static_cast<int>(p < 0 ? 0 : (p > cap ? cap : p));
+  return within >> a.page_shift << a.page_shift;
 }
 
 // Sequence s of the plan: with a shared prefix, 0 is the prefix under all rows

@@ -191,11 +191,13 @@ def shared_prefix_attention(q, key_pages, value_pages, prefix_pages, prefix_leng
     """paged_attention of sequences that begin with the same prefix, whose keys and
     values are read once for all rows.
 
-    Slots below prefix_length (int64 [1], on device) are those of prefix_pages
-    (int32 [P], on device) for every sequence; the others go by page_table as
-    ever, whose entries of whole pages below the prefix's end are not used.
-    lengths counts the prefix. A prefix_length outside the slots of prefix_pages
-    is taken as the nearest one within.
+    The whole pages below prefix_length (int64 [1], on device) are those of
+    prefix_pages (int32 [P], on device) for every sequence, and page_table's
+    entries of them are not used. The other slots go by page_table as ever, the
+    prefix's last ones among them where it ends inside a page: each sequence has
+    them in the page that holds its own next ones. lengths counts the prefix. A
+    prefix_length outside the slots of prefix_pages is taken as the nearest one
+    within.
     """
     if prefix_pages.dim() != 1 or prefix_pages.dtype != torch.int32 or prefix_pages.numel() < 1 \
             or not prefix_pages.is_contiguous():
