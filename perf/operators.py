@@ -167,10 +167,9 @@ def prepare(case, seed):
     else:
         state.q = normal(total, heads, D, std=2.0).to(torch.bfloat16)
     if case["kind"] == "prefix":
-        # Whole pages are shared; the rest of a prefix that ends inside a page lies
-        # in pages of the sequences' own.
-        state.prefix_pages = table[0, :max(1, shared)].contiguous()
-        state.prefix_length = torch.tensor([shared * page], device=DEVICE)
+        # The prefix's last page may hold the first sequence's own slots too.
+        state.prefix_pages = table[0, :-(-prefix // page)].contiguous()
+        state.prefix_length = torch.tensor([prefix], device=DEVICE)
     return state
 
 
