@@ -544,6 +544,13 @@ __device__ __forceinline__ late_args_t late_args() {
 // in them stays one.
 __device__ __forceinline__ float share(float x) { return fmaxf(__builtin_amdgcn_exp2f(x), 1.2e-38f); }
 
+// The reference that a finished state without a finite score is said to have: then it
+// sums to nothing (no slot seen, or scores of -inf alone) or to NaN (a NaN score), and
+// the sums go into those of other states like any. Whether a row sees a slot is told
+// by its position: from 0 on it sees its own. So a row of NaN scores, or of -inf ones
+// alone (0 / 0), gives NaN, and only a row that sees nothing gives zeros.
+constexpr float kNoScore = -3.402823466e38f;
+
 // The reference that weights are taken against moves only when a row's maximum has
 // outgrown it by 2^kSlack: the sums have room for that, and most tiles then leave
 // the accumulators alone (5000-token prompt 250 -> 240 us).
@@ -716,17 +723,15 @@ __device__ __forceinline__ void attend_few(const PagedArgs& a, const Item& it, c
     }
     __syncthreads();
     for (int c = wave; c < 16 && 16 * n + c < it.rows; c += 4) {
-      const float M = fmaxf(fmaxf(wm[0][c], wm[1][c]), fmaxf(wm[2][c], wm[3][c]));
+      const float M = fmaxf(fmaxf(fmaxf(wm[0][c], wm[1][c]), fmaxf(wm[2][c], wm[3][c])), kNoScore);
       float L = 0.f, x = 0.f, y = 0.f;
-      if (M != -INFINITY) {
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const float f = share(wm[w][c] - M);
-          const float2 o = *reinterpret_cast<const float2*>(wacc + (w * 16 + c) * kRowFloats + 2 * lane);
-          L = fmaf(f, wl[w][c], L);
-          x = fmaf(f, o.x, x);
-          y = fmaf(f, o.y, y);
-        }
+      for (int w = 0; w < 4; ++w) {
+        const float f = share(wm[w][c] - M);
+        const float2 o = *reinterpret_cast<const float2*>(wacc + (w * 16 + c) * kRowFloats + 2 * lane);
+        L = fmaf(f, wl[w][c], L);
+        x = fmaf(f, o.x, x);
+        y = fmaf(f, o.y, y);
       }
       if (it.part >= 0) {
         const long row = it.part + 16 * n + c;
@@ -735,7 +740,7 @@ __device__ __forceinline__ void attend_few(const PagedArgs& a, const Item& it, c
       } else {
         int tr, hr;
         row_of(la->G, it, kFewRows, 16 * n + c, tr, hr);
-        const float inv = M == -INFINITY ? 0.f : 1.0f / L;
+        const float inv = it.p0 + (tr - it.t0) < 0 ? 0.f : 1.0f / L;
         *reinterpret_cast<uint32_t*>(la->out + tr * la->o_st + hr * la->o_sh + 2 * lane) = pack_bf2(x * inv, y * inv);
       }
     }
@@ -987,17 +992,16 @@ __device__ __forceinline__ void attend_many(const PagedArgs& a, const Item& it, 
   for (int n = 0; n < 2; ++n) {
     const int r = 32 * wave + 16 * n + col;
     if (r >= it.rows) continue;
-    const bool none = m[n] == -INFINITY;
     if (it.part >= 0) {
       const long row = it.part + r;
 #pragma unroll
       for (int j = 0; j < 8; ++j)
         *reinterpret_cast<f32x4_t*>(la->part + row * D + 16 * j + 4 * quad) = acc[n][j];
-      if (quad == 0) la->ml[row] = make_float2(none ? -INFINITY : m[n] * la->scale2, sum[n][0]);
+      if (quad == 0) la->ml[row] = make_float2(fmaxf(m[n] * la->scale2, kNoScore), sum[n][0]);
     } else {
       int t, h;
       row_of(la->G, it, kManyRows, r, t, h);
-      const float inv = none ? 0.f : 1.0f / sum[n][0];
+      const float inv = it.p0 + (t - it.t0) < 0 ? 0.f : 1.0f / sum[n][0];
       bf16_t* dst = la->out + t * la->o_st + h * la->o_sh + 4 * quad;
 #pragma unroll
       for (int j = 0; j < 8; ++j)
@@ -1061,10 +1065,10 @@ __global__ __launch_bounds__(kBlock) void paged_merge_kernel(PagedArgs a) {
     if (!split) return;
     if (j >= a.B) continue;
     const PlanEntry own = a.plan[j + (shared ? 1 : 0)];
-    const int64_t from = a.starts[j], to = a.starts[j + 1], end = a.starts[a.B];
+    const int64_t from = a.starts[j], to = a.starts[j + 1], end = a.starts[a.B], length = a.lengths[j];
     if (!own.chunks || t < from || t >= to) continue;  // with chunks, starts rise
     const int kvh = h / a.G;
-    float M = -INFINITY, L = 0.f;
+    float M = kNoScore, L = 0.f;
     f32x4_t o = {0.f, 0.f, 0.f, 0.f};
     auto fold = [&](const PlanEntry& p, int token, int tokens) {
       const int r = token * a.G + h % a.G;
@@ -1073,7 +1077,7 @@ __global__ __launch_bounds__(kBlock) void paged_merge_kernel(PagedArgs a) {
       const long step = static_cast<long>(a.Hkv) * p.stride;
       for (int c0 = 0; c0 < p.chunks; c0 += kWave) {
         const int n = p.chunks - c0 < kWave ? p.chunks - c0 : kWave;
-        const float2 ml = lane < n ? a.ml[row + (c0 + lane) * step] : make_float2(-INFINITY, 0.f);
+        const float2 ml = lane < n ? a.ml[row + (c0 + lane) * step] : make_float2(kNoScore, 0.f);
         constexpr int U = 8;
         f32x4_t x[U];
         auto fetch = [&](int c) {
@@ -1085,9 +1089,7 @@ __global__ __launch_bounds__(kBlock) void paged_merge_kernel(PagedArgs a) {
         };
         fetch(0);
         const float mb = fmaxf(M, wave_max(ml.x));
-        if (mb == -INFINITY) continue;
-        const float f0 = share(M - mb);
-        const float f = ml.x == -INFINITY ? 0.f : share(ml.x - mb);
+        const float f0 = share(M - mb), f = share(ml.x - mb);
         M = mb;
         L = fmaf(L, f0, wave_sum(f * ml.y));
         o *= f0;
@@ -1096,7 +1098,7 @@ __global__ __launch_bounds__(kBlock) void paged_merge_kernel(PagedArgs a) {
           for (int u = 0; u < U; ++u) {
             const int at = c + 2 * u + half;
             const float g = __shfl(f, at < n ? at : 0, kWave);
-            if (at < n && g != 0.f) o += x[u] * g;  // a chunk that saw nothing wrote no weights
+            if (at < n) o += x[u] * g;
           }
           c += 2 * U;
           if (c >= n) break;
@@ -1108,7 +1110,8 @@ __global__ __launch_bounds__(kBlock) void paged_merge_kernel(PagedArgs a) {
     if (shared) fold(a.plan[0], t, static_cast<int>(end));
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], 32, kWave);
-    const float inv = M == -INFINITY ? 0.f : 1.0f / L;
+    const Span s = make_span(from, to, length, a.T, a.table_pages << a.page_shift);
+    const float inv = s.p0 + (t - s.t0) < 0 ? 0.f : 1.0f / L;
     if (half == 0)
       *reinterpret_cast<uint2*>(a.out + t * a.o_st + h * a.o_sh + dim) =
           make_uint2(pack_bf2(o[0] * inv, o[1] * inv), pack_bf2(o[2] * inv, o[3] * inv));

@@ -176,7 +176,8 @@ def paged_attention(q, key_pages, value_pages, page_table, query_starts, lengths
     new tokens' keys and values already in their pages (norm_rope_paged). With
     `window` a row at position p sees the last `window` slots, p - window + 1 to
     p, and the first `sinks` slots of the sequence, however far back. Rows that
-    see nothing get zeros. `out`, when given, is a bf16 view shaped like q.
+    see nothing get zeros; a NaN in a query or in a visible key gives NaN. `out`,
+    when given, is a bf16 view shaped like q.
     """
     if window < 0 or sinks < 0:
         raise ValueError("window and sinks must not be negative")

@@ -547,7 +547,8 @@ int htn_norm_rope_paged(const void* q, int64_t q_st, const void* k, int64_t k_st
 /* out[t, h] = softmax(q . k / sqrt(128)) v over the slots s <= p, p the row's
  * position; with window > 0 of these only s > p - window and s < sinks. Rows
  * that see nothing get zeros. Infinities and NaN in slots that a row does not
- * see do not reach it. q and out rows at t * st + h * sh elements (q strides
+ * see do not reach it; a row that sees a score of NaN or +inf, or none but
+ * -inf, is NaN. q and out rows at t * st + h * sh elements (q strides
  * multiples of 8 from a 16-byte aligned base, out strides of 4 from an 8-byte
  * aligned one). scratch: htn_paged_attention_scratch_bytes bytes, no initial
  * contents, 16-byte aligned. */

@@ -1,4 +1,5 @@
-"""The paged operators where a prefix ends inside a page.
+"""The paged operators where a prefix ends inside a page, and where queries or keys are
+NaN or infinite.
 
 Outputs are compared with the definition in 64 bits, bounds as in test_gpu_paged.py: an
 output is off by 2 * 2^-8 sum_s p_s |v_s| for weights and their sum rounded to bf16 and by
@@ -9,11 +10,11 @@ import math
 import pytest
 import torch
 
-from hackthenorth_amd.kernels.paged import shared_prefix_attention
+from hackthenorth_amd.kernels.paged import paged_attention, shared_prefix_attention
 from test_gpu_paged import D, Batch
 
 pytestmark = pytest.mark.gpu
-INF = float("inf")
+INF, NAN = float("inf"), float("nan")
 
 
 def definition(b, window=0, sinks=0):
@@ -67,3 +68,61 @@ def test_prefix_that_ends_inside_a_page(new, lengths, heads, kv_heads, page, pre
             pages[-1] = last
         again = shared_prefix_attention(q, keys, values, pages.cuda(), length, table, starts, dev_lengths)
         assert torch.equal(again, got)
+
+
+# Rows of blocks that split the slots and of those that split the rows, whole and in
+# chunks: single tokens, verify rows, prompts; a window; a prefix.
+BATCHES = [([1, 1], [1, 100], 8, 4, 0, 0), ([5, 1], [60, 33], 16, 4, 0, 0), ([1, 5], [3000, 900], 16, 4, 0, 0),
+           ([100], [110], 8, 4, 0, 0), ([200, 1], [2000, 700], 8, 4, 0, 0), ([64], [4000], 4, 1, 0, 0),
+           ([1, 40], [2000, 1500], 8, 4, 100, 0), ([1, 5, 1], [700, 620, 513], 8, 4, 0, 512),
+           ([90, 1], [400, 300], 8, 4, 0, 200)]
+
+
+def run(b, window, prefix):
+    q, keys, values, table, starts, lengths = b.cuda()
+    if prefix:
+        return shared_prefix_attention(q, keys, values, table[0, :prefix // 16].contiguous(),
+                                       torch.tensor([prefix], device="cuda"), table, starts, lengths)
+    return paged_attention(q, keys, values, table, starts, lengths, window=window)
+
+
+@pytest.mark.parametrize("value", [NAN, INF, -INF])
+@pytest.mark.parametrize("new,lengths,heads,kv_heads,window,prefix", BATCHES)
+def test_nonfinite_queries(new, lengths, heads, kv_heads, window, prefix, value):
+    """A NaN or infinity in a query makes its row NaN and no other one."""
+    b = Batch(new, lengths, heads, kv_heads, 16, prefix=prefix)
+    b.q[0, 1, 7] = b.q[-1, heads - 1] = b.q[len(b.q) // 2, 0, 100] = value
+    check(b, run(b, window, prefix), window)
+
+
+@pytest.mark.parametrize("value", [NAN, INF, -INF])
+@pytest.mark.parametrize("new,lengths,heads,kv_heads,window,prefix", BATCHES)
+def test_nonfinite_keys(new, lengths, heads, kv_heads, window, prefix, value):
+    """Keys of one slot, of all the slots of some chunk or of the whole sequence: a row that
+    sees a score of NaN or +inf is NaN; scores of -inf weigh nothing, and where a row sees
+    nothing else it is NaN."""
+    def spoil(b, i, slots):
+        b.keys[b.table[i].long()[slots // 16], kv_heads - 1, slots % 16] = value
+    for i, length in enumerate(lengths):
+        for slots in (torch.tensor([length - 1]), torch.tensor([0]), torch.arange(min(length, 300)),
+                      torch.arange(length // 2, length), torch.arange(length)):
+            b = Batch(new, lengths, heads, kv_heads, 16, prefix=prefix)
+            b.q = b.q.abs() + 0.01
+            spoil(b, i, slots)
+            check(b, run(b, window, prefix), window)
+
+
+def test_rows_that_see_nothing_stay_zero():
+    """NaN queries of rows before slot 0 or with a length that does not fit."""
+    for new, bad in (([3, 2], 1), ([3, 2], -4), ([3, 90], 40), ([3, 90], 1 << 40)):
+        b = Batch(new, [600, 200], 8, 4, 16)
+        q, keys, values, table, starts, lengths = b.cuda()
+        lengths[1] = bad
+        q[3:] = NAN
+        out = paged_attention(q, keys, values, table, starts, lengths)
+        seen = max(0, bad) if bad <= 200 else 0
+        assert bool((out[3:len(q) - seen] == 0).all()) and bool(out[len(q) - seen:].isnan().all())
+        assert bool(out[:3].isfinite().all())
+        prefixed = shared_prefix_attention(q, keys, values, table[0, :8].contiguous(),
+                                           torch.tensor([128], device="cuda"), table, starts, lengths)
+        assert torch.equal(prefixed.isnan(), out.isnan()) and bool((prefixed[3:len(q) - seen] == 0).all())
