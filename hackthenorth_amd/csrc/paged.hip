@@ -541,8 +541,9 @@ __device__ __forceinline__ late_args_t late_args() {
 }
 
 // What earlier sums weigh against later ones, 2^x. Not 0, so that an infinity or a NaN
-// in them stays one.
-__device__ __forceinline__ float share(float x) { return fmaxf(__builtin_amdgcn_exp2f(x), 1.2e-38f); }
+// in them stays one, but the least that fp32 holds: sums of any finite V then come to
+// less than 5e-7 where they should not count.
+__device__ __forceinline__ float share(float x) { return fmaxf(__builtin_amdgcn_exp2f(x), 0x1p-149f); }
 
 // The reference that a finished state without a finite score is said to have: then it
 // sums to nothing (no slot seen, or scores of -inf alone) or to NaN (a NaN score), and

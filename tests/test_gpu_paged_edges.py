@@ -1,5 +1,5 @@
-"""The paged operators where a prefix ends inside a page, and where queries or keys are
-NaN or infinite.
+"""The paged operators where a prefix ends inside a page, where queries, keys or weights
+are NaN or infinite, and where V is huge.
 
 Outputs are compared with the definition in 64 bits, bounds as in test_gpu_paged.py: an
 output is off by 2 * 2^-8 sum_s p_s |v_s| for weights and their sum rounded to bf16 and by
@@ -126,3 +126,17 @@ def test_rows_that_see_nothing_stay_zero():
         prefixed = shared_prefix_attention(q, keys, values, table[0, :8].contiguous(),
                                            torch.tensor([128], device="cuda"), table, starts, lengths)
         assert torch.equal(prefixed.isnan(), out.isnan()) and bool((prefixed[3:len(q) - seen] == 0).all())
+
+
+@pytest.mark.parametrize("new,lengths,heads,kv_heads,window,prefix", [c for c in BATCHES if c[1][0] > 200])
+def test_huge_values_without_weight(new, lengths, heads, kv_heads, window, prefix):
+    """Slots whose scores lie some 450 below the others' weigh e^-450: V of 2^112 there
+    leaves the outputs alone."""
+    b = Batch(new, lengths, heads, kv_heads, 16, prefix=prefix)
+    b.q = torch.full_like(b.q, 2.0)
+    for i, length in enumerate(lengths):
+        slots = torch.arange(0, length // 2)
+        where = b.table[i].long()[slots // 16], slots % 16
+        b.keys[where[0], :, where[1]] = -20.0
+        b.values[where[0], :, where[1]] = 2.0 ** 112
+    check(b, run(b, window, prefix), window)
