@@ -16,7 +16,9 @@ query_starts must not fall and must lie within [0, T], else the attention writes
 nothing. A sequence whose length is negative or past its table's slots sees
 nothing and stores nothing. Page ids outside the pool read as zeros and are not
 written, and entries of slots that no row sees are never used. Rows of no
-sequence (behind the last one in a padded batch) are left as they were.
+sequence (behind the last one in a padded batch) are left as they were in `out`;
+without `out` they, and all rows of a batch whose starts are refused, hold
+whatever the new tensor's memory held.
 """
 import functools
 
@@ -91,7 +93,7 @@ def _scratch_bytes(tokens, batch, heads, kv_heads, shared):
 
 
 def norm_rope_paged(q, k, v, q_norm, k_norm, cos, sin, key_pages, value_pages, page_table,
-                    query_starts, lengths):
+                    query_starts, lengths, out=None):
     """QK-norm and RoPE of the new tokens; k and v into their pages. Returns q [T, Hq, 128].
 
     q, k and v are [T, heads, 128] views with packed heads (slices of the packed
@@ -99,6 +101,8 @@ def norm_rope_paged(q, k, v, q_norm, k_norm, cos, sin, key_pages, value_pages, p
     turns position p (zeros past the last). q_norm/k_norm are RMSNorms over the
     head; None leaves both unnormalised. Norm and rotation run in fp32 and round
     once, where norm_rope_cache keeps the reference's rounding after every step.
+    `out`, when given, receives q: contiguous bf16 [T, Hq, 128], apart from the
+    inputs' memory.
     """
     (shape, q_st), (k_shape, k_st), (v_shape, v_st) = _rows(q, "q"), _rows(k, "k"), _rows(v, "v")
     tokens, heads, dim = shape
@@ -129,9 +133,12 @@ def norm_rope_paged(q, k, v, q_norm, k_norm, cos, sin, key_pages, value_pages, p
     if pool_heads != kv_heads:
         raise ValueError("page pools must have k's heads")
     batch, row_st, row_pages = _check_batch(page_table, query_starts, lengths)
+    if out is not None and (out.shape != shape or out.dtype is not _BF16 or not out.is_contiguous()):
+        raise ValueError("out must be contiguous bf16 shaped like q")
     index = _place(q, k, v, q_gain, k_gain, cos, sin, key_pages, value_pages, page_table,
-                   query_starts, lengths)
-    out = torch.empty_like(q, memory_format=_PACKED)
+                   query_starts, lengths, out)
+    if out is None:
+        out = torch.empty_like(q, memory_format=_PACKED)
     _launch("htn_norm_rope_paged", index, q.data_ptr(), q_st[0], k.data_ptr(), k_st[0],
             v.data_ptr(), v_st[0], _lib.ptr(q_gain), _lib.ptr(k_gain), q_eps, k_eps,
             cos.data_ptr(), sin.data_ptr(), table_st[0], table_shape[0], kind is torch.float32,

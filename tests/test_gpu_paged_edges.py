@@ -1,5 +1,5 @@
 """The paged operators where a prefix ends inside a page, where queries, keys or weights
-are NaN or infinite, and where V is huge.
+are NaN or infinite, where V is huge, and with padded batches.
 
 Outputs are compared with the definition in 64 bits, bounds as in test_gpu_paged.py: an
 output is off by 2 * 2^-8 sum_s p_s |v_s| for weights and their sum rounded to bf16 and by
@@ -10,8 +10,9 @@ import math
 import pytest
 import torch
 
-from hackthenorth_amd.kernels.paged import paged_attention, shared_prefix_attention
-from test_gpu_paged import D, Batch
+from hackthenorth_amd.kernels.paged import (norm_rope_paged, paged_attention,
+                                            shared_prefix_attention)
+from test_gpu_paged import D, Batch, tables
 
 pytestmark = pytest.mark.gpu
 INF, NAN = float("inf"), float("nan")
@@ -140,3 +141,54 @@ def test_huge_values_without_weight(new, lengths, heads, kv_heads, window, prefi
         b.keys[where[0], :, where[1]] = -20.0
         b.values[where[0], :, where[1]] = 2.0 ** 112
     check(b, run(b, window, prefix), window)
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_padded_rows_keep_what_out_held(captured):
+    """Append and attention of a padded batch into the caller's tensors: rows before the
+    first sequence and behind the last as they were, then with refused starts all of them."""
+    b = Batch([3, 1, 40], [100, 33, 64], 8, 4, 16, poison=0.0)
+    _, keys, values, table, starts, lengths = b.cuda()
+    packed = torch.randn(60, 16, D, device="cuda").to(torch.bfloat16)
+    q, k, v = packed[:, :8], packed[:, 8:12], packed[:, 12:]
+    cos, sin = (t.cuda() for t in tables(128, torch.float32))
+    starts += 5
+    rest = (keys, values, table[0, :1].contiguous(), torch.zeros(1, dtype=torch.int64, device="cuda"), table,
+            starts, lengths)
+    rows, outs = slice(5, 49), [torch.empty(60, 8, D, device="cuda", dtype=torch.bfloat16) for _ in range(3)]
+
+    def step(outs):
+        turned = norm_rope_paged(q, k, v, None, None, cos, sin, keys, values, table, starts, lengths, out=outs[0])
+        assert turned is outs[0]
+        paged_attention(turned, keys, values, table, starts, lengths, out=outs[1])
+        shared_prefix_attention(turned, *rest, out=outs[2])
+    own = norm_rope_paged(q, k, v, None, None, cos, sin, keys, values, table, starts, lengths)
+    want = [own, paged_attention(own, keys, values, table, starts, lengths)]
+    want.append(shared_prefix_attention(own, *rest))
+
+    def again():
+        step(outs)
+    if captured:
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            step(outs)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            step(outs)
+        again = graph.replay
+    for fill in (7.0, -3.0):
+        for out in outs:
+            out.fill_(fill)
+        again()
+        torch.cuda.synchronize()
+        for out, one in zip(outs, want):
+            assert torch.equal(out[rows], one[rows])
+            assert bool((out[:5] == fill).all()) and bool((out[49:] == fill).all())
+    starts[2] = 200
+    for out in outs:
+        out.fill_(1.0)
+    again()
+    torch.cuda.synchronize()
+    assert all(bool((out == 1.0).all()) for out in outs[1:])
