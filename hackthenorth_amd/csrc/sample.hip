@@ -9,8 +9,9 @@
 // of the token's distance to the bin's edge (half a unit, 2^-34 of the weight, is
 // lost a token), and a bin's sum times 2^11 exp of the edge, rounded, over the
 // bins. Borders between tokens so fall where 64-bit sums put them but for some
-// 2^-34 of a token's weight. Tokens 32 nats and more below the largest weigh
-// nothing.
+// 2^-34 of a token's weight, and for the tokens 32 nats and more below the largest,
+// which weigh nothing: e^-32 of the largest weight each, 524160 of them 2^-27. A
+// draw of 24 bits never falls among them.
 //
 //   1. every chunk of a row: its largest logit;
 //   2. every chunk: the count and weight of its tokens in 1024 bins below the

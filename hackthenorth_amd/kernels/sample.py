@@ -7,7 +7,10 @@ top_k; the shortest leading part that holds top_p of the weight so far; those th
 weigh at least min_p times the largest. The answer is the first token whose
 cumulative weight passes `uniform` times the weight kept. Random numbers come from
 the caller, so a draw can be repeated, and weights are summed as 64-bit integers, so
-a row's token does not depend on the batch it is drawn in.
+a row's token does not depend on the batch it is drawn in. They are exact to 2^-34 of a
+token's weight, but tokens 32 temperatures and more below the largest logit weigh
+nothing: all of them together at most vocab e^-32 of the largest weight (7e-9 at 524160,
+the most a row may have).
 """
 import functools
 

@@ -588,8 +588,10 @@ int htn_shared_prefix_attention(const void* q, int64_t q_st, int64_t q_sh, const
  * that weigh at least min_p times the largest. The answer is the first token
  * whose cumulative weight passes uniform[r] times the weight kept. T not above
  * 0 gives the first token. Weights are summed as integers (2^-34 of a token's
- * weight at most is lost), so a row's token is the same in every batch. NaN and -inf
- * are masked, +inf tokens share all the weight; a row with nothing left gives
+ * weight at most is lost), so a row's token is the same in every batch. Tokens 32
+ * T and more below the largest logit weigh nothing: sums may be short by up to
+ * vocab e^-32 of the largest weight (7e-9 at most), below what a uniform number
+ * of 24 bits resolves, so no draw is lost to them. NaN and -inf are masked, +inf tokens share all the weight; a row with nothing left gives
  * -1. Each setting is a device array with one value per row, or NULL and the
  * value after it for all rows. scratch: htn_sample_scratch_bytes bytes, no
  * initial contents, 16-byte aligned. No counterpart in the reference, which
