@@ -569,9 +569,10 @@ constexpr float kSlack = 8.f;
 // Bound by the K/V stream: each wave stages its own 16 slots through LDS, two tiles
 // ahead, and waits for nobody. 16 sequences of 32 + 8 heads, 24 K slots in all
 // (98 MB): 21 us, 4.7 TB/s; three of 30 K slots (306 MB): 50 us, 6.1 TB/s.
-// Against the waves splitting the rows (attend_many), 8 sequences of 5 rows, 20 a
-// head, at up to 4096 slots take 29.9 us to 31.1, 32 of them 47 to 53; with 32 rows
-// a head the two are within 8% either way, and this one keeps 16 bits of a weight.
+// Against the waves splitting the rows (attend_many), 8 sequences of up to 5 rows, 20 a
+// head, at up to 4096 slots (101 MB) take 30.1 us to 29.8, 32 of them (382 MB) 93.7 to
+// 100; with 32 rows a head the two are within 8% either way, and this one keeps 16 bits
+// of a weight.
 template <int NT>
 __device__ __forceinline__ void attend_few(const PagedArgs& a, const Item& it, const Slots& sl,
                                            const int32_t* table, const int* rowpos,
@@ -1053,7 +1054,8 @@ __global__ __launch_bounds__(kBlock, 2) void paged_attention_kernel(PagedArgs a)
 // over the chunks of the row's own slots and, where one is shared, of the prefix.
 // A lane first holds a chunk's (m, l); then each half of the wave takes every
 // other chunk's row, four dims a lane, eight chunks' loads in flight. A launch of
-// 4-6 us, 2048 blocks at most; one that finds nothing split ends at once.
+// 4-6 us, 2048 blocks at most, and 4.0-4.6 where the prompt's 160000 rows are not split:
+// its waves end at their first row, once they have the plan.
 __global__ __launch_bounds__(kBlock) void paged_merge_kernel(PagedArgs a) {
   const int lane = threadIdx.x & 63, half = lane >> 5, dim = 4 * (lane & 31);
   const int split = a.plan[0].split;

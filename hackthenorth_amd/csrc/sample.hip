@@ -28,8 +28,8 @@
 //
 // One row of 151936 bf16 logits takes 23.7 us: five launches of 3, 5, 6, 4.5 and
 // 7 us, each a chain of loads, scans and barriers. 64 such rows in fp32 (39 MB) take
-// 51: 6.5, 15, 9, 11 and 10.5 us, the second bound by 64-bit arithmetic (two or four
-// copies of the bins change nothing). A row of equal logits takes 165. Before the
+// 51: 6, 15, 9, 11 and 10.5 us, the second bound by its arithmetic (vector instructions
+// issue in 83% of the cycles; two or four copies of the bins change nothing). A row of equal logits takes 165. Before the
 // steps were as short, steps 2 + 3 and 4 + 5 in one launch each, by the row's last
 // block, gained one row 0.8 us and cost 64 rows 12; steps 3 + 4, each block planning
 // for itself, gained 1.6 and cost 2.

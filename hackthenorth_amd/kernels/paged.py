@@ -199,6 +199,11 @@ def shared_prefix_attention(q, key_pages, value_pages, prefix_pages, prefix_leng
     """paged_attention of sequences that begin with the same prefix, whose keys and
     values are read once for all rows.
 
+    For single tokens and a few rows a sequence, which K/V reads bound. Every row's
+    two parts, prefix and own, are written and merged, 520 bytes a part and head, so
+    prompts are faster by paged_attention (8 chunks of up to 512 tokens behind 2048
+    slots, 32 heads: 173 us, here 272).
+
     The whole pages below prefix_length (int64 [1], on device) are those of
     prefix_pages (int32 [P], on device) for every sequence, and page_table's
     entries of them are not used. The other slots go by page_table as ever, the

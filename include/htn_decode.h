@@ -566,7 +566,8 @@ int htn_paged_attention(const void* q, int64_t q_st, int64_t q_sh, const void* k
  * within [0, prefix_count * page_size]) are those of prefix_pages for every
  * sequence: their K and V are read once for all rows, and the sequences' own
  * table entries of these pages are not used. Slots from there on, the prefix's
- * last ones among them where it ends inside a page, go by page_table. */
+ * last ones among them where it ends inside a page, go by page_table. Each row
+ * is merged from partials of both parts: for few rows a sequence. */
 int htn_shared_prefix_attention(const void* q, int64_t q_st, int64_t q_sh, const void* keys,
                                 const void* values, int64_t pages, int64_t page_size,
                                 const int32_t* prefix_pages, int64_t prefix_count,
